@@ -47,6 +47,27 @@ uint32_t qw_rope_tables_blocks_host(const uint32_t *block_h, const uint32_t *blo
                                     const uint32_t *text_before, uint32_t n_blocks,
                                     float *cos_out, float *sin_out);
 
+/* NEW: frequencies [rotary_dim / 2] and magnitude for qw_gpu_rotary_bf16: theta^(-2i / rotary_dim),
+ * stretched for contexts `factor` times the trained length.  LINEAR: divided by factor.  THETA: theta
+ * grown so that the slowest pair is divided by factor and the fastest kept.  PARTS: pairs that turn
+ * more than 32 times within trained_length kept, those that turn less than once divided, the others
+ * between; the magnitude is 0.1 ln(factor) + 1 (1 otherwise).  Returns 0 on arguments out of range. */
+enum {
+    QW_ROTARY_SCALE_NONE = 0,
+    QW_ROTARY_SCALE_LINEAR = 1,
+    QW_ROTARY_SCALE_THETA = 2,
+    QW_ROTARY_SCALE_PARTS = 3
+};
+int qw_rotary_frequencies_host(uint32_t rotary_dim, float theta, uint32_t scaling, float factor,
+                               uint32_t trained_length, float *frequencies, float *magnitude);
+
+/* NEW: bf16 weights [output_dim, input_dim] to the 4-bit form of qw_gpu_linear_w4_bf16, without zero
+ * points: packed [output_dim, input_dim / 8], scales bf16 [output_dim, input_dim / group].  Of each
+ * group the scale is its largest magnitude over 7, rounded to bf16, and q the nearest whole number of
+ * w / scale (ties to even).  Returns 0 on arguments out of range or a weight that is not finite. */
+int qw_w4_quantize_host(const uint16_t *weight, uint32_t output_dim, uint32_t input_dim, uint32_t group,
+                        uint32_t *packed, uint16_t *scales);
+
 #ifdef __cplusplus
 }
 #endif

@@ -189,6 +189,82 @@ int qw_gpu_attn_block_causal_bounded_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                                           uint32_t head_dim, const uint32_t *text_len,
                                           uint32_t text_pad, float scale);
 
+/* ---- a text tower that is served token by token --------------------------
+ * The reference's tower runs whole prompts; these continue them.
+ *
+ * Rotary positions for grouped heads: q [tokens, heads, head_dim], k [tokens,
+ * kv_heads, head_dim] (key_input and key_output both NULL: q alone).  Of each head
+ * the first rotary_dim elements are rotated in pairs, (2i, 2i+1) for
+ * QW_ROTARY_NEIGHBOURS or (i, i + rotary_dim/2) for QW_ROTARY_HALVES:
+ *   (a, b) <- magnitude * (a cos(pf) - b sin(pf), a sin(pf) + b cos(pf))
+ * with p = positions[token] (U32) and f = frequencies[i] (F32 [rotary_dim/2]; see
+ * qw_rotary_frequencies_host for the scalings of long contexts); the rest of the head
+ * is copied.  p * f is reduced in 64 bits: positions may be anything.  head_dim even, up
+ * to 512.  Each output may be its own input. */
+enum { QW_ROTARY_NEIGHBOURS = 0, QW_ROTARY_HALVES = 1 };
+int qw_gpu_rotary_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_tensor *key_output,
+                       const h3_gpu_tensor *query_input, const h3_gpu_tensor *key_input,
+                       const h3_gpu_tensor *positions, const h3_gpu_tensor *frequencies,
+                       uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                       uint32_t rotary_dim, uint32_t layout, float magnitude);
+
+/* A paged K/V cache of a batch of sequences, shared by the two ops below:
+ *   key_pages, value_pages  pools [pages, page_rows, kv_heads, head_dim]; page_rows a
+ *                 power of two, 16 to 4096
+ *   page_table    U32 [batch, table_width]: cache row r of sequence b is row
+ *                 r % page_rows of page page_table[b][r / page_rows]; entries past a
+ *                 sequence's last page are not read
+ *   token_start   U32 [batch + 1]: sequence b's new tokens are rows token_start[b] ..
+ *                 token_start[b+1] (none is fine) of the token-major tensors, which have
+ *                 `tokens` rows; rows of no sequence, such as padding behind the last, are
+ *                 neither read nor written
+ *   cache_len     U32 [batch]: cache rows, the new tokens included; these are the last
+ * All three are device tensors, so a step captured into a graph is replayed with other
+ * lengths after writing them.  A page outside the pool, a token range outside the tensors
+ * or a length beyond the page table is clamped and h3_gpu_submit returns 0 with the place.
+ * A sequence with more new tokens than cache rows has no row for the first of them: they
+ * are not appended and attend to nothing.
+ *
+ * The new tokens of one layer: q rotated into query_output (may be query_input), k rotated
+ * and v copied into their cache rows.  Rotation as in qw_gpu_rotary_bf16; positions NULL: a
+ * token's cache row.  A pool row that two tokens name is written by either. */
+int qw_gpu_rotary_append_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_tensor *key_pages,
+                              h3_gpu_tensor *value_pages, const h3_gpu_tensor *query_input,
+                              const h3_gpu_tensor *key_new, const h3_gpu_tensor *value_new,
+                              const h3_gpu_tensor *positions, const h3_gpu_tensor *frequencies,
+                              const h3_gpu_tensor *page_table, const h3_gpu_tensor *token_start,
+                              const h3_gpu_tensor *cache_len, uint32_t batch, uint32_t tokens,
+                              uint32_t table_width, uint32_t page_rows, uint32_t heads,
+                              uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim,
+                              uint32_t layout, float magnitude);
+
+/* Attention of the new tokens over the cache, from single tokens to chunks of a prompt:
+ * a token sees its sequence's cache rows up to its own.  query, output [tokens, heads, 128];
+ * grouped heads as in qw_gpu_flash_sdpa_prefix_bf16; scale positive.  A token that sees
+ * nothing stores zeros.  Cache rows past a sequence's end may hold anything; the values of
+ * its new tokens must be finite where an earlier one's result is wanted.  max_new: new
+ * tokens of the longest sequence, which only chooses the kernels (a sequence may have
+ * more).  The first call makes a workspace of the context: run the op once before
+ * capturing it. */
+int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,
+                                const h3_gpu_tensor *key_pages, const h3_gpu_tensor *value_pages,
+                                const h3_gpu_tensor *page_table, const h3_gpu_tensor *token_start,
+                                const h3_gpu_tensor *cache_len, uint32_t batch, uint32_t tokens,
+                                uint32_t max_new, uint32_t table_width, uint32_t page_rows,
+                                uint32_t heads, uint32_t kv_heads, uint32_t head_dim, float scale);
+
+/* Linear layer with 4-bit weights: output[rows, output_dim] = bf16(bias + input . w^T),
+ * w[o][c] = scales[o][c / group] * (q[o][c] - zeros[o][c / group]).
+ *   weight  U32 [output_dim, input_dim / 8]: q of column 8j + i in bits 4i .. 4i+3 of word j
+ *   scales  bf16 [output_dim, input_dim / group]; zeros the same (any values), or NULL: 8
+ *   bias    bf16 [output_dim] or NULL
+ * group: 32, 64 or a multiple of 128, and input_dim whole groups; any output_dim, up to
+ * 2^19 rows.  qw_w4_quantize_host makes such weights of bf16 ones. */
+int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                          const h3_gpu_tensor *weight, const h3_gpu_tensor *scales,
+                          const h3_gpu_tensor *zeros, const h3_gpu_tensor *bias, uint32_t rows,
+                          uint32_t input_dim, uint32_t output_dim, uint32_t group);
+
 /* Context bound to an explicit CUDA device. */
 h3_gpu *qw_gpu_create_on_device(int device, char *error, size_t error_size);
 int qw_gpu_device(const h3_gpu *gpu);

@@ -117,6 +117,10 @@ _SIGNATURES = {
     "qw_gpu_attn_block_causal_bf16": (
         C.c_int, [c_gpu, c_tensor, c_tensor, c_tensor, c_tensor, c_tensor, u32, u32, u32, u32, u32,
                   C.c_void_p, u32, f32]),
+    "qw_gpu_rotary_bf16": (C.c_int, [c_gpu] + [c_tensor] * 6 + [u32] * 6 + [f32]),
+    "qw_gpu_rotary_append_bf16": (C.c_int, [c_gpu] + [c_tensor] * 11 + [u32] * 9 + [f32]),
+    "qw_gpu_paged_attention_bf16": (C.c_int, [c_gpu] + [c_tensor] * 7 + [u32] * 8 + [f32]),
+    "qw_gpu_linear_w4_bf16": (C.c_int, [c_gpu] + [c_tensor] * 6 + [u32] * 4),
     "qw_gpu_device": (C.c_int, [c_gpu]),
     "qw_gpu_tensor_device_ptr": (C.c_void_p, [c_tensor]),
     "qw_gpu_stream": (C.c_void_p, [c_gpu]),
@@ -156,6 +160,8 @@ _SIGNATURES = {
     "qw_pipe_rope_tables_blocks": (
         C.c_int, [c_gpu, C.c_void_p, C.c_void_p, C.c_void_p, u32, C.POINTER(c_tensor),
                   C.POINTER(c_tensor), C.c_char_p, size_t]),
+    "qw_rotary_frequencies_host": (C.c_int, [u32, f32, u32, f32, u32, C.c_void_p, C.c_void_p]),
+    "qw_w4_quantize_host": (C.c_int, [C.c_void_p, u32, u32, u32, C.c_void_p, C.c_void_p]),
     "qw_rope_tables_host": (u32, [u32, u32, u32, C.c_void_p, C.c_void_p]),
     "qw_rope_tables_blocks_host": (u32, [C.c_void_p, C.c_void_p, C.c_void_p, u32, C.c_void_p, C.c_void_p]),
 }

@@ -392,11 +392,11 @@ static inline int make_map_2d(CUtensorMap *map, const void *base, uint32_t rows,
 // Launch behind the stream's last kernel with the programmatic dependency described at
 // grid_wait(), in clusters of `cluster` CTAs.
 template <typename... Params, typename... Args>
-static inline int launch(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem,
+static inline int launch(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
                          int cluster, cudaStream_t stream, const Args &...args) {
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute attrs[2];
-    config.gridDim = dim3(grid);
+    config.gridDim = grid;
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;

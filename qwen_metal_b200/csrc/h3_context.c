@@ -210,6 +210,7 @@ void h3_gpu_free(h3_gpu *gpu) {
     cudaSetDevice(gpu->device);
     if (gpu->stream) cudaStreamSynchronize(gpu->stream);
     if (gpu->scratch) cudaFree(gpu->scratch);
+    if (gpu->paged_work) cudaFree(gpu->paged_work);
     if (gpu->status_host) cudaFreeHost(gpu->status_host);
     if (gpu->chain_start) cudaEventDestroy(gpu->chain_start);
     if (gpu->chain_stop) cudaEventDestroy(gpu->chain_stop);
@@ -563,6 +564,15 @@ int h3_gpu_submit(h3_gpu *gpu) {
                          "row index %u, outside the modulation tensor; block 0 was used instead",
                          gpu->status_host[0], gpu->status_host[1], gpu->status_host[2],
                          gpu->status_host[3]);
+        else if (gpu->status_host[0] == QWCU_STATUS_BAD_CACHE)
+            qw_set_error(gpu, "CUDA kernel reported status %u: %s of sequence %u is %u",
+                         gpu->status_host[0],
+                         gpu->status_host[1] == QWCU_BAD_PAGE          ? "a page outside the pool,"
+                         : gpu->status_host[1] == QWCU_BAD_TOKEN_START ? "the token range is not one "
+                                                                         "of the tensor's: the end"
+                                                                       : "the cache length exceeds the "
+                                                                         "page table: that",
+                         gpu->status_host[2], gpu->status_host[3]);
         else
             qw_set_error(gpu,
                          "CUDA kernel reported status %u (where 0x%x, tile %u, block 0x%x): a "

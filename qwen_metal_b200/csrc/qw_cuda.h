@@ -22,8 +22,10 @@ typedef void *qwcu_stream;
 enum {
     QWCU_STATUS_OK = 0,
     QWCU_STATUS_WAIT_TIMEOUT = 1, /* status[1] = role<<16 | barrier id, status[2] = tile */
-    QWCU_STATUS_BAD_ARGUMENT = 2
+    QWCU_STATUS_BAD_ARGUMENT = 2,
+    QWCU_STATUS_BAD_CACHE = 3 /* status[1] = one of the below, [2] = sequence, [3] = value */
 };
+enum { QWCU_BAD_PAGE = 1, QWCU_BAD_TOKEN_START = 2, QWCU_BAD_CACHE_LEN = 3 };
 #define QWCU_STATUS_WORDS 8
 
 /* Geometry + mask description shared by every attention kernel.
@@ -229,6 +231,72 @@ typedef struct {
 } qwcu_linear_plan;
 int qwcu_linear_sm100_plan(uint32_t m, uint32_t n, uint32_t n_outputs, int sm_count,
                            qwcu_linear_plan *plan);
+
+/* A paged K/V cache and its batch of new tokens (layouts in cuda/qw_paged.cuh). */
+typedef struct {
+    const uint32_t *page_table;  /* [batch][table_width] */
+    const uint32_t *token_start; /* [batch + 1] */
+    const uint32_t *cache_len;   /* [batch] */
+    uint32_t batch;
+    uint32_t table_width;
+    uint32_t page_shift; /* log2 of the rows of a page */
+    uint32_t pool_pages;
+    uint32_t *status;
+} qwcu_cache_args;
+
+/* Rotary positions (cuda/qw_rotary.cu): q [tokens][heads][head_dim] and, unless k_in is
+ * NULL, k [tokens][kv_heads][head_dim].  With v_in the rotated k and the copied v go to the
+ * cache's pools k_out / v_out [pages][page rows][kv_heads][head_dim], and positions may be
+ * NULL: a token's position is its cache row. */
+typedef struct {
+    const void *q_in;
+    const void *k_in;
+    const void *v_in;
+    void *q_out;
+    void *k_out;
+    void *v_out;
+    const uint32_t *positions;
+    const float *frequencies; /* [rotary_dim / 2] */
+    uint32_t tokens, heads, kv_heads, head_dim, rotary_dim;
+    int half; /* pairs (i, i + rotary_dim / 2) instead of (2i, 2i + 1) */
+    float magnitude;
+    qwcu_cache_args cache;
+} qwcu_rotary_args;
+
+int qwcu_rotary_launch(const qwcu_rotary_args *args, int sm_count, qwcu_stream stream);
+
+/* Attention of new tokens over a paged cache: q, out [tokens][heads][128], pools
+ * [pages][page rows][kv_heads][128]. */
+typedef struct {
+    const void *q;
+    const void *k_pages;
+    const void *v_pages;
+    void *out;
+    uint32_t tokens, heads, kv_heads;
+    uint32_t max_new; /* tokens of the longest sequence, as the caller says (choice of kernels only) */
+    float scale;
+    qwcu_cache_args cache;
+    void *workspace; /* qwcu_paged_workspace_bytes(sm_count) bytes, zeroed once */
+} qwcu_paged_args;
+
+/* A host constant of the device: nothing of a call's sizes is in it. */
+size_t qwcu_paged_workspace_bytes(int sm_count);
+/* Sequences of few query rows: streams K and V through registers (cuda/qw_paged_few.cu). */
+int qwcu_paged_few_launch(const qwcu_paged_args *args, int sm_count, qwcu_stream stream);
+
+/* y[rows][n] = x[rows][k] . w[n][k]^T (+ bias), w = scale * (q - zero) with 4-bit q, eight to
+ * a word, and a scale (and zero) per `group` columns (cuda/qw_linear_w4.cu). */
+typedef struct {
+    const void *x;
+    const uint32_t *w;  /* [n][k / 8] */
+    const void *scales; /* bf16 [n][k / group] */
+    const void *zeros;  /* the same, or NULL: 8 */
+    const void *bias;   /* bf16 [n] or NULL */
+    void *y;
+    uint32_t rows, k, n, group;
+} qwcu_linear_w4_args;
+
+int qwcu_linear_w4_launch(const qwcu_linear_w4_args *args, int sm_count, qwcu_stream stream);
 
 /* Device properties needed by the host side. */
 int qwcu_device_sm_count(int device);

@@ -45,6 +45,8 @@ struct h3_gpu {
     /* Scratch for the pre-scaled query of the h3 causal variant; grows on demand. */
     void *scratch;
     size_t scratch_bytes;
+    /* The paged attention's partial results and arrival counters (zero between launches). */
+    void *paged_work;
 };
 
 struct qw_gpu_graph {

@@ -131,3 +131,73 @@ int qw_pipe_rope_tables_blocks(h3_gpu *gpu, const uint32_t *block_h, const uint3
     return tables_to_device(gpu, rows, cos_host, sin_host, rope_cos, rope_sin, error, error_size,
                             "rope blocks: build failed");
 }
+
+/* Frequencies of the rotated pairs.  The scalings for contexts longer than the trained one are all in
+ * them and in the factor on cosine and sine: LINEAR divides every frequency by `factor`; THETA takes
+ * theta * factor^(d / (d - 2)), so that the fastest pair stays and the slowest is divided by it; PARTS
+ * leaves pairs that turn more than 32 times within the trained length, divides those that turn less
+ * than once, goes over linearly in the turns between, and grows the factor with ln(factor). */
+int qw_rotary_frequencies_host(uint32_t rotary_dim, float theta, uint32_t scaling, float factor,
+                               uint32_t trained_length, float *frequencies, float *magnitude) {
+    if (!rotary_dim || rotary_dim % 2 || !(theta > 0.0f) || !isfinite(theta) || !frequencies ||
+        !magnitude || scaling > QW_ROTARY_SCALE_PARTS)
+        return 0;
+    if (scaling != QW_ROTARY_SCALE_NONE && (!(factor >= 1.0f) || !isfinite(factor))) return 0;
+    if (scaling == QW_ROTARY_SCALE_PARTS && !trained_length) return 0;
+    if (scaling == QW_ROTARY_SCALE_THETA && rotary_dim < 4) return 0;
+    const double d = rotary_dim;
+    double base = theta;
+    if (scaling == QW_ROTARY_SCALE_THETA) base *= pow(factor, d / (d - 2.0));
+    *magnitude = scaling == QW_ROTARY_SCALE_PARTS ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+    for (uint32_t i = 0; i < rotary_dim / 2; i++) {
+        double f = pow(base, -2.0 * i / d);
+        if (scaling == QW_ROTARY_SCALE_LINEAR) f /= factor;
+        if (scaling == QW_ROTARY_SCALE_PARTS) {
+            double keep = (trained_length * f / 6.283185307179586 - 1.0) / (32.0 - 1.0);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f = f * keep + f / factor * (1.0 - keep);
+        }
+        frequencies[i] = (float)f;
+    }
+    return 1;
+}
+
+static float widened(uint16_t bits) {
+    union { uint32_t u; float f; } x = {(uint32_t)bits << 16};
+    return x.f;
+}
+static uint16_t narrowed(float value) { /* to nearest even; value is finite */
+    union { float f; uint32_t u; } x = {value};
+    return (uint16_t)((x.u + 0x7fffu + ((x.u >> 16) & 1u)) >> 16);
+}
+
+/* Symmetric 4-bit weights: of each group of columns the scale is its largest magnitude over 7, rounded
+ * to bf16, and q the nearest whole number (ties to even) of w / scale within -8 .. 7, plus 8. */
+int qw_w4_quantize_host(const uint16_t *weight, uint32_t output_dim, uint32_t input_dim, uint32_t group,
+                        uint32_t *packed, uint16_t *scales) {
+    if (!weight || !packed || !scales || !output_dim || !input_dim ||
+        !(group == 32 || group == 64 || (group && group % 128 == 0)) || input_dim % group)
+        return 0;
+    const size_t groups = (size_t)output_dim * (input_dim / group);
+    for (size_t g = 0; g < groups; g++) {
+        const uint16_t *w = weight + g * group;
+        float most = 0.0f;
+        for (uint32_t i = 0; i < group; i++) {
+            const float v = fabsf(widened(w[i]));
+            if (!isfinite(v)) return 0;
+            if (v > most) most = v;
+        }
+        scales[g] = narrowed(most / 7.0f);
+        const float scale = widened(scales[g]);
+        for (uint32_t i = 0; i < group; i += 8) {
+            uint32_t word = 0;
+            for (uint32_t j = 0; j < 8; j++) {
+                float q = scale > 0.0f ? rintf(widened(w[i + j]) / scale) : 0.0f;
+                q = q < -8.0f ? -8.0f : q > 7.0f ? 7.0f : q;
+                word |= (uint32_t)((int)q + 8) << (4 * j);
+            }
+            packed[(g * group + i) / 8] = word;
+        }
+    }
+    return 1;
+}

@@ -141,3 +141,46 @@ int qw_gpu_qkv_norm_rope_bf16(h3_gpu *gpu, h3_gpu_tensor *query_out, h3_gpu_tens
     args.bound_out = score_bound ? (float *)score_bound->dev : NULL;
     return launch_linear(gpu, &args, "Qwen QKV norm+rope");
 }
+
+/* NEW: output[rows, output_dim] = bf16(bias + input . w^T) with 4-bit weights, w = scale * (q - zero)
+ * per group of columns. */
+int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
+                          const h3_gpu_tensor *weight, const h3_gpu_tensor *scales,
+                          const h3_gpu_tensor *zeros, const h3_gpu_tensor *bias, uint32_t rows,
+                          uint32_t input_dim, uint32_t output_dim, uint32_t group) {
+    if (!gpu) return 0;
+    if (!rows || !input_dim || !output_dim || !(group == 32 || group == 64 || (group && group % 128 == 0)) ||
+        input_dim % group || rows > (1u << 19)) {
+        qw_set_error(gpu, "4-bit linear: unsupported geometry (groups of 32, 64 or a multiple of 128 "
+                          "columns, whole groups, at most 2^19 rows)");
+        return 0;
+    }
+    size_t input_count = (size_t)rows * input_dim, output_count = (size_t)rows * output_dim;
+    size_t weight_count = (size_t)output_dim * (input_dim / 8);
+    size_t group_count = (size_t)output_dim * (input_dim / group);
+    if (!qw_require_dtype(gpu, input, input_count, H3_GPU_BF16, "4-bit linear input") ||
+        !qw_require_dtype(gpu, weight, weight_count, H3_GPU_U32, "4-bit linear weight") ||
+        !qw_require_dtype(gpu, scales, group_count, H3_GPU_BF16, "4-bit linear scales") ||
+        (zeros && !qw_require_dtype(gpu, zeros, group_count, H3_GPU_BF16, "4-bit linear zeros")) ||
+        (bias && !qw_require_dtype(gpu, bias, output_dim, H3_GPU_BF16, "4-bit linear bias")) ||
+        !qw_require_dtype(gpu, output, output_count, H3_GPU_BF16, "4-bit linear output"))
+        return 0;
+    if (!qw_require_command(gpu)) return 0;
+    const h3_gpu_tensor *all[] = {input, weight, scales, zeros, bias, output};
+    for (int i = 0; i < 6; i++)
+        if (all[i] && all[i]->owner->device != gpu->device) {
+            qw_set_error(gpu, "4-bit linear: a tensor lies on another device");
+            return 0;
+        }
+    if (output == input || output == scales || output == zeros || output == bias) {
+        qw_set_error(gpu, "4-bit linear: the output is also an input");
+        return 0;
+    }
+    if (!qw_bind(gpu)) return 0;
+    qwcu_linear_w4_args args = {input->dev, weight->dev, scales->dev, zeros ? zeros->dev : NULL,
+                                bias ? bias->dev : NULL, output->dev, rows, input_dim, output_dim,
+                                group};
+    int rc = qwcu_linear_w4_launch(&args, qwcu_device_sm_count(gpu->device), gpu->stream);
+    qw_count_launch(gpu, rc, "4-bit linear");
+    return rc == 0;
+}
