@@ -42,7 +42,7 @@ struct Params {
     const uint16_t *q, *k_pages, *v_pages;
     uint16_t *out;
     uint32_t heads, kv_heads, share;  // share: query heads of a kv head
-    uint32_t skip_rows;               // sequences with more query rows are another kernel's
+    uint32_t most_rows;               // sequences with more query rows are another kernel's
     float scale_log2;
     float *partials;     // two of each CTA
     uint32_t *counters;  // one of each CTA, zero between launches
@@ -82,7 +82,7 @@ template <int kRows>
 __device__ __forceinline__ Work work_of(const Params &p, const paged::Sequence &s) {
     const unsigned long long rows = (unsigned long long)s.fresh * p.share;
     Work w;
-    w.row_tiles = rows > p.skip_rows ? 0u : (uint32_t)((rows + kRows - 1) / kRows);
+    w.row_tiles = rows > p.most_rows ? 0u : (uint32_t)((rows + kRows - 1) / kRows);
     w.tiles = max(1u, ((uint32_t)s.length + kKeys - 1) / kKeys);  // (no key: zeros are still written)
     return w;
 }
@@ -370,12 +370,13 @@ unsigned most_ctas(int sm_count) { return (unsigned)(sm_count > 0 ? sm_count : 1
 
 }  // namespace
 
-extern "C" size_t qwcu_paged_workspace_bytes(int sm_count) {
+extern "C" size_t qwcu_paged_few_workspace_bytes(int sm_count) {
     const size_t ctas = most_ctas(sm_count);
     return ctas * 2 * kPartial * sizeof(float) + ctas * sizeof(uint32_t);
 }
 
-extern "C" int qwcu_paged_few_launch(const qwcu_paged_args *a, int sm_count, qwcu_stream stream_) {
+extern "C" int qwcu_paged_few_launch(const qwcu_paged_args *a, uint32_t most_rows, void *workspace,
+                                     int sm_count, qwcu_stream stream_) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!a->tokens || !a->cache.batch || !a->heads || !a->kv_heads || a->heads % a->kv_heads ||
         a->cache.page_shift < 4 || !a->cache.pool_pages)
@@ -389,13 +390,13 @@ extern "C" int qwcu_paged_few_launch(const qwcu_paged_args *a, int sm_count, qwc
     p.heads = a->heads;
     p.kv_heads = a->kv_heads;
     p.share = a->heads / a->kv_heads;
-    p.skip_rows = 0xffffffffu;
+    p.most_rows = most_rows;
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    p.partials = static_cast<float *>(a->workspace);
+    p.partials = static_cast<float *>(workspace);
     p.counters = reinterpret_cast<uint32_t *>(p.partials + (size_t)ctas * 2 * kPartial);
     p.cache = {a->cache.page_table, a->cache.token_start, a->cache.cache_len, a->cache.batch, a->tokens,
                a->cache.table_width, a->cache.page_shift, a->cache.pool_pages, a->cache.status};
-    const bool narrow = (unsigned long long)a->max_new * p.share <= 8;
+    const bool narrow = (unsigned long long)a->max_new * p.share <= 8 || most_rows <= 8;
     return sm100::launch(narrow ? qw_paged_few_kernel<1> : qw_paged_few_kernel<2>,
                          narrow ? ctas : ctas / kCtasPerSm * 2, kThreads, 0, 1, stream, p);
 }

@@ -276,13 +276,22 @@ typedef struct {
     uint32_t max_new; /* tokens of the longest sequence, as the caller says (choice of kernels only) */
     float scale;
     qwcu_cache_args cache;
-    void *workspace; /* qwcu_paged_workspace_bytes(sm_count) bytes, zeroed once */
+    /* Bounded-wait exercise, as in qwcu_attn_args (the kernel for chunks only). */
+    long long wait_cycles;
+    int withhold_from;
 } qwcu_paged_args;
 
-/* A host constant of the device: nothing of a call's sizes is in it. */
-size_t qwcu_paged_workspace_bytes(int sm_count);
-/* Sequences of few query rows: streams K and V through registers (cuda/qw_paged_few.cu). */
-int qwcu_paged_few_launch(const qwcu_paged_args *args, int sm_count, qwcu_stream stream);
+/* Sequences of up to most_rows query rows (new tokens x heads / kv_heads): K and V go through
+ * registers (cuda/qw_paged_few.cu).  Workspaces are of one size for all calls on a device; this one
+ * is zeroed when it is made. */
+size_t qwcu_paged_few_workspace_bytes(int sm_count);
+int qwcu_paged_few_launch(const qwcu_paged_args *args, uint32_t most_rows, void *workspace,
+                          int sm_count, qwcu_stream stream);
+/* Sequences of at least least_rows query rows, heads / kv_heads <= 128: tcgen05
+ * (cuda/qw_paged_chunk.cu), one or two kernels. */
+size_t qwcu_paged_chunk_workspace_bytes(int sm_count);
+int qwcu_paged_chunk_launch(const qwcu_paged_args *args, uint32_t least_rows, void *workspace,
+                            int sm_count, qwcu_stream stream, int *launched);
 
 /* y[rows][n] = x[rows][k] . w[n][k]^T (+ bias), w = scale * (q - zero) with 4-bit q, eight to
  * a word, and a scale (and zero) per `group` columns (cuda/qw_linear_w4.cu). */

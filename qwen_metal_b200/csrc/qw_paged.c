@@ -198,8 +198,8 @@ int qw_gpu_rotary_append_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_t
     return launch_rotary(gpu, &args, what);
 }
 
-/* The paged attention's workspace: of one size for every call on a device, made by the first. */
-static void *paged_workspace(h3_gpu *gpu) {
+/* The paged attention's workspaces: of one size for every call on a device, made by the first. */
+static char *paged_workspace(h3_gpu *gpu, size_t few_bytes, size_t chunk_bytes) {
     if (gpu->paged_work) return gpu->paged_work;
     if (gpu->capturing) {
         qw_set_error(gpu, "paged attention: run it once before capturing it into a graph (it makes its "
@@ -207,20 +207,23 @@ static void *paged_workspace(h3_gpu *gpu) {
         gpu->chain_failed = 1;
         return NULL;
     }
-    size_t bytes = qwcu_paged_workspace_bytes(qwcu_device_sm_count(gpu->device));
     void *block = NULL;
-    if (cudaMallocAsync(&block, bytes, gpu->stream) != cudaSuccess) {
+    if (cudaMallocAsync(&block, few_bytes + chunk_bytes, gpu->stream) != cudaSuccess) {
         cudaGetLastError();
-        qw_set_error(gpu, "cannot allocate %zu bytes of workspace", bytes);
+        qw_set_error(gpu, "cannot allocate %zu bytes of workspace", few_bytes + chunk_bytes);
         return NULL;
     }
-    if (!qw_cuda_ok(gpu, cudaMemsetAsync(block, 0, bytes, gpu->stream), "workspace")) {
+    if (!qw_cuda_ok(gpu, cudaMemsetAsync(block, 0, few_bytes, gpu->stream), "workspace")) {
         cudaFreeAsync(block, gpu->stream);
         return NULL;
     }
     gpu->paged_work = block;
     return block;
 }
+
+/* Query rows (new tokens x query heads of a kv head) up to which a sequence goes to the kernel for
+ * few: one of its units. */
+#define QW_PAGED_FEW_ROWS 16u
 
 int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,
                                 const h3_gpu_tensor *key_pages, const h3_gpu_tensor *value_pages,
@@ -262,9 +265,27 @@ int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu
     args.kv_heads = kv_heads;
     args.max_new = max_new;
     args.scale = scale;
-    args.workspace = paged_workspace(gpu);
-    if (!args.workspace) return 0;
-    int rc = qwcu_paged_few_launch(&args, qwcu_device_sm_count(gpu->device), gpu->stream);
-    qw_count_launch(gpu, rc, what);
+    args.wait_cycles = gpu->attn_wait_cycles;
+    args.withhold_from = gpu->attn_withhold_tile;
+    const int sms = qwcu_device_sm_count(gpu->device);
+    const size_t few_bytes = (qwcu_paged_few_workspace_bytes(sms) + 255) / 256 * 256;
+    char *workspace = paged_workspace(gpu, few_bytes, qwcu_paged_chunk_workspace_bytes(sms));
+    if (!workspace) return 0;
+    /* Each kernel skips the other's sequences; one sequence alone needs no second kernel. */
+    const uint32_t share = heads / kv_heads;
+    const int chunks = share <= 128 && (uint64_t)max_new * share > QW_PAGED_FEW_ROWS;
+    int rc = 0;
+    if (chunks) {
+        int launched;
+        rc = qwcu_paged_chunk_launch(&args, batch == 1 ? 0u : QW_PAGED_FEW_ROWS + 1u,
+                                     workspace + few_bytes, sms, gpu->stream, &launched);
+        for (; launched > (rc ? 0 : 1); launched--) qw_count_launch(gpu, 0, what);
+        qw_count_launch(gpu, rc, what);
+    }
+    if (!rc && (!chunks || batch > 1)) {
+        rc = qwcu_paged_few_launch(&args, chunks ? QW_PAGED_FEW_ROWS : UINT32_MAX, workspace, sms,
+                                   gpu->stream);
+        qw_count_launch(gpu, rc, what);
+    }
     return rc == 0;
 }

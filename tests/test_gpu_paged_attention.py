@@ -245,3 +245,21 @@ def test_agrees_with_the_whole_prompt(gpu):
         d = np.abs(R.wide(got) - R.wide(want[at:at + n]))
         assert (d <= 2 * (R.HALF_STEP * np.abs(R.wide(got)) + (R.HALF_STEP + 2.0 ** -11) * size)).all()
         at += n
+
+
+@pytest.mark.parametrize("new,length", [(300, 1500), (40, 1500), (100, 6000)])
+def test_bounded_waits_run_out_cleanly(gpu, new, length):
+    """Key tiles from the second on stay away (nothing is in flight): the waits behind them run out, the
+    submit says so and the next call is right."""
+    rng = np.random.default_rng(12)
+    cache = R.Cache(rng, [new], [length], 32, 2)
+    q = R.random_bf16(rng, cache.tokens, 8, 128)
+    gpu.check(gpu.lib.qw_gpu_debug_attention_waits(gpu.handle, 2_000_000, 1))
+    try:
+        ok, error, _ = attend(gpu, cache, q)
+    finally:
+        gpu.lib.qw_gpu_debug_attention_waits(gpu.handle, 0, 0)
+    assert not ok and "wait ran out" in error
+    ok, error, got = attend(gpu, cache, q)
+    assert ok, error
+    check(cache, got, q)
