@@ -360,9 +360,9 @@ qw_attn_sm100_kernel(const __grid_constant__ CUtensorMap map_q,
         uint8_t *stage = smem_q + (size_t)sub * kTileBytes;
         const uint32_t tile_row0 = split ? row0 : row0 + (uint32_t)sub * kTileM;
         const int pad_lo = p.text_pad ? (int)p.text_len[b] : 0, pad_hi = (int)p.text_pad;
-        // (Captured by name: with [&] the epilogue's spills grew from 12 to 36 bytes and four short layers
-        // took 0.8 % longer.)
-        const auto store = [&p, stage, tid_in_group, tile_row0, b, h](uint32_t tmem_own, uint32_t tmem_other, float w_own, float w_other,
+        // (Captured by name: with [&] the kernel spills 36 bytes instead of 12.)
+        const auto store = [&p, stage, tid_in_group, tile_row0, b, h](
+                               uint32_t tmem_own, uint32_t tmem_other, float w_own, float w_other,
                                float inv, float, float) __attribute__((always_inline)) {
             const int warp_in_group = tid_in_group >> 5;
             const uint32_t warp_row0 = tile_row0 + (uint32_t)warp_in_group * 32u;

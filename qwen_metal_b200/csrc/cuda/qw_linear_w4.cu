@@ -22,8 +22,8 @@
 
 namespace {
 
-constexpr int kWarps = 8;
 constexpr uint32_t kChunk = 128;  // columns of a warp's step
+
 
 struct Params {
     const uint16_t *x;
@@ -31,6 +31,7 @@ struct Params {
     const uint16_t *scales, *zeros, *bias;
     uint16_t *y;
     uint32_t rows, k, n, group;
+    uint32_t per_group;  // groups of more than 128 columns: 2^32 over their chunks, rounded up
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -41,103 +42,167 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Columns i and i + 4 of a word, less 8, as a pair of bf16: 0x4300 | q is 128 + q.
+// Columns i and i + 4 of a word as a pair of bf16: 0x4300 | q is 128 + q.
 __device__ __forceinline__ uint32_t pair_of(uint32_t word, int i) {
     uint32_t r;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(word >> (4 * i)));
-    const __nv_bfloat162 minus = __halves2bfloat162(__ushort_as_bfloat16(0xc308), __ushort_as_bfloat16(0xc308));
-    const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&r), minus);
-    return *reinterpret_cast<const uint32_t *>(&v);
+    return r;
 }
 
 __device__ __forceinline__ float widened(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
 
-// The four words of an output that a lane has of a chunk.  Groups of 128 columns and more: words
-// 4t .. 4t + 3, one load; narrower ones, whose columns must not meet in one MMA: words t, 4 + t, ...
-template <bool kWide>
-__device__ __forceinline__ void load_words(uint32_t (&w)[4], const uint32_t *row, uint32_t words,
-                                           uint32_t chunk, uint32_t t) {
-    if constexpr (kWide) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row + chunk * 16) + t);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else {
+__device__ __forceinline__ uint4 load_stream(const uint32_t *p) {
+    uint4 v;  // weights pass once; L1 is for x
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+// Word i of lane t becomes word t of lane i, in each quad.
+__device__ __forceinline__ void transpose_quad(uint32_t (&w)[4], uint32_t t) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t at = chunk * 16 + 4 * j + t;
-            w[j] = at < words ? __ldg(row + at) : 0u;
+    for (int step = 1; step <= 2; step <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i & step) continue;
+            const uint32_t mine = (t & step) ? w[i] : w[i | step];
+            const uint32_t theirs = __shfl_xor_sync(0xffffffffu, mine, step);
+            if (t & step) w[i] = theirs;
+            else w[i | step] = theirs;
         }
     }
 }
 
-// kFold: words of a lane after which a group ends (1: 32 columns, 2: 64, 4: 128 and more).
-template <int kTilesN, int kTilesM, int kFold, bool kZeros>
-__global__ void __launch_bounds__(kWarps * 32) qw_linear_w4_kernel(const Params p) {
+// Packed fp32 pairs (one issue slot for two).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// Asks for [p, p + bytes) in L2, less what is not whole 16-byte pieces of it.
+__device__ __forceinline__ void prefetch_l2(const void *p, size_t bytes) {
+    const uintptr_t from = ((uintptr_t)p + 15) & ~(uintptr_t)15, to = ((uintptr_t)p + bytes) & ~(uintptr_t)15;
+    if (from < to)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t)(to - from))
+                     : "memory");
+}
+
+// What a lane holds of a chunk: words 4t .. 4t + 3 of its outputs, a scale and a zero point.
+template <int kTilesM>
+struct Stage {
+    uint4 w[kTilesM][2];
+    uint16_t s[kTilesM][2], z[kTilesM][2];
+};
+
+// kTilesN: 8 rows of x each; kTilesM: 16 outputs each.  kFold: words of a lane after which a group ends
+// (1: 32 columns, 2: 64, 4: 128 and more).  kAhead: chunks of a warp in flight.
+template <int kWarps, int kTilesN, int kTilesM, int kFold, bool kZeros, int kAhead, int kCtas>
+__global__ void __launch_bounds__(kWarps * 32, kCtas) qw_linear_w4_kernel(const Params p) {
     constexpr int kRows = 8 * kTilesN, kOutputs = 16 * kTilesM;
     constexpr bool kWide = kFold == 4;
     __shared__ float sums[kWarps][kRows][kOutputs + 1];
-    sm100::grid_launch_dependents();
-    sm100::grid_wait();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t out0 = blockIdx.x * kOutputs, row0 = blockIdx.y * kRows;
-    const uint32_t words = p.k / 8, groups = p.k / p.group, chunks = (p.k + kChunk - 1) / kChunk;
-
-    // Outputs past the end are the last one's once more and not stored.
+    const uint32_t words = p.k / 8, groups = p.k / p.group, parts = p.k / 32;
+    const uint32_t chunks = (p.k + kChunk - 1) / kChunk;
+    // The CTA's weights and scales lie together.  Asking for them in L2 reads nothing that could be
+    // out of date later, so it may run under the kernel before.
+    sm100::grid_launch_dependents();
+    if (threadIdx.x == 0) {
+        const uint32_t outs = min((uint32_t)kOutputs, p.n - out0);
+        prefetch_l2(p.w + (size_t)out0 * words, (size_t)outs * words * 4);
+        prefetch_l2(p.scales + (size_t)out0 * groups, (size_t)outs * groups * 2);
+        if constexpr (kZeros) prefetch_l2(p.zeros + (size_t)out0 * groups, (size_t)outs * groups * 2);
+    }
+    // Rows and outputs past the end are the last one's once more, and not stored: loads need no
+    // conditions.  So are chunks past the end, which are loaded ahead and not used.
     const uint32_t *w_row[kTilesM][2];
-    size_t s_row[kTilesM][2];
+    const uint16_t *s_row[kTilesM][2];
+    const size_t zeros_from_scales = kZeros ? (size_t)(p.zeros - p.scales) : 0;
 #pragma unroll
     for (int m = 0; m < kTilesM; ++m)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const uint32_t o = min(out0 + 16 * m + 8 * r + g, p.n - 1);
             w_row[m][r] = p.w + (size_t)o * words;
-            s_row[m][r] = (size_t)o * groups;
+            s_row[m][r] = p.scales + (size_t)o * groups;
         }
-    float total[kTilesM][kTilesN][4] = {};
-    uint32_t next[kTilesM][2][4];
-    if (warp < chunks) {
+    const uint16_t *x_row[kTilesN];
+#pragma unroll
+    for (int n = 0; n < kTilesN; ++n)
+        x_row[n] = p.x + (size_t)min(row0 + 8 * n + g, p.rows - 1) * p.k;
+
+    using Ring = Stage<kTilesM>;
+    const auto fetch = [&](Ring &st, uint32_t chunk) __attribute__((always_inline)) {
+        chunk = min(chunk, chunks - 1);
+        uint32_t at, group;
+        if constexpr (kWide) {
+            at = chunk * 16 + 4 * t;
+            group = p.per_group ? __umulhi(chunk, p.per_group) : chunk;
+        } else {
+            const uint32_t part = min(chunk * 4 + t, parts - 1);  // of 32 columns
+            at = part * 4;
+            group = part / kFold;
+        }
 #pragma unroll
         for (int m = 0; m < kTilesM; ++m)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) load_words<kWide>(next[m][r], w_row[m][r], words, warp, t);
-    }
-    for (uint32_t chunk = warp; chunk < chunks; chunk += kWarps) {
+            for (int r = 0; r < 2; ++r) {
+                st.w[m][r] = load_stream(w_row[m][r] + at);
+                st.s[m][r] = __ldg(s_row[m][r] + group);
+                if constexpr (kZeros) st.z[m][r] = __ldg(s_row[m][r] + zeros_from_scales + group);
+            }
+    };
+    float2 total[kTilesM][kTilesN][2] = {};
+    const auto consume = [&](const Ring &st, uint32_t chunk) __attribute__((always_inline)) {
+        uint4 x[kTilesN][4];
+#pragma unroll
+        for (int n = 0; n < kTilesN; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t column =
+                    kWide ? chunk * kChunk + 32 * t + 8 * j : min(chunk * 4 + j, parts - 1) * 32 + 8 * t;
+                x[n][j] = __ldg(reinterpret_cast<const uint4 *>(x_row[n] + column));
+            }
         uint32_t w[kTilesM][2][4];
 #pragma unroll
         for (int m = 0; m < kTilesM; ++m)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[m][r][j] = next[m][r][j];
-                if (chunk + kWarps < chunks)
-                    load_words<kWide>(next[m][r], w_row[m][r], words, chunk + kWarps, t);
+                w[m][r][0] = st.w[m][r].x, w[m][r][1] = st.w[m][r].y;
+                w[m][r][2] = st.w[m][r].z, w[m][r][3] = st.w[m][r].w;
+                // Narrow groups' columns must not meet in one MMA with another group's.
+                if constexpr (!kWide) transpose_quad(w[m][r], t);
             }
         float acc[kTilesM][kTilesN][4], of_x[kTilesN][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (!kWide && chunk * 4 + j >= parts) break;
             if (j % kFold == 0) {
 #pragma unroll
-                for (int n = 0; n < kTilesN; ++n) {
+                for (int n = 0; n < kTilesN; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) of_x[n][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) {
+                        of_x[n][i] = 0.0f;
 #pragma unroll
-                    for (int m = 0; m < kTilesM; ++m)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
-                }
+                        for (int m = 0; m < kTilesM; ++m) acc[m][n][i] = 0.0f;
+                    }
             }
-            const uint32_t column = chunk * kChunk + (kWide ? 32 * t + 8 * j : 32 * j + 8 * t);
             uint32_t b[kTilesN][4];
 #pragma unroll
             for (int n = 0; n < kTilesN; ++n) {
-                const uint32_t row = row0 + 8 * n + g;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < p.rows && column < p.k)
-                    v = __ldg(reinterpret_cast<const uint4 *>(p.x + (size_t)row * p.k + column));
-                b[n][0] = __byte_perm(v.x, v.z, 0x5410);
-                b[n][1] = __byte_perm(v.x, v.z, 0x7632);
-                b[n][2] = __byte_perm(v.y, v.w, 0x5410);
-                b[n][3] = __byte_perm(v.y, v.w, 0x7632);
+                b[n][0] = __byte_perm(x[n][j].x, x[n][j].z, 0x5410);
+                b[n][1] = __byte_perm(x[n][j].x, x[n][j].z, 0x7632);
+                b[n][2] = __byte_perm(x[n][j].y, x[n][j].w, 0x5410);
+                b[n][3] = __byte_perm(x[n][j].y, x[n][j].w, 0x7632);
             }
+            const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -149,34 +214,46 @@ __global__ void __launch_bounds__(kWarps * 32) qw_linear_w4_kernel(const Params 
                     for (int n = 0; n < kTilesN; ++n)
                         mma(acc[m][n], a, b[n][2 * half], b[n][2 * half + 1]);
                 }
-                if constexpr (kZeros) {
-                    const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-                    for (int n = 0; n < kTilesN; ++n)
-                        mma(of_x[n], ones, b[n][2 * half], b[n][2 * half + 1]);
-                }
+                for (int n = 0; n < kTilesN; ++n)
+                    mma(of_x[n], ones, b[n][2 * half], b[n][2 * half + 1]);
             }
             if (j % kFold == kFold - 1) {
-                // (a group past the last column has sums of zero)
-                const uint32_t group =
-                    min(kWide ? chunk * kChunk / p.group : (chunk * kChunk + 32 * j) / p.group, groups - 1);
 #pragma unroll
                 for (int m = 0; m < kTilesM; ++m)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float s = widened(__ldg(p.scales + s_row[m][r] + group));
-                        float z = 0.0f;
-                        if constexpr (kZeros) z = widened(__ldg(p.zeros + s_row[m][r] + group)) - 8.0f;
+                        // (a narrow group's scale is with the lane whose load it was)
+                        uint32_t s = st.s[m][r], z = kZeros ? st.z[m][r] : 0u;
+                        if constexpr (!kWide) {
+                            if constexpr (kZeros) s |= z << 16;
+                            s = __shfl_sync(0xffffffffu, s, j, 4);
+                            if constexpr (kZeros) z = s >> 16;
+                        }
+                        const float scale = __uint_as_float(s << 16);
+                        const float less = kZeros ? -128.0f - __uint_as_float(z << 16) : -136.0f;
+                        const float2 scale2 = make_float2(scale, scale), less2 = make_float2(less, less);
 #pragma unroll
-                        for (int n = 0; n < kTilesN; ++n)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                float v = acc[m][n][2 * r + i];
-                                if constexpr (kZeros) v = fmaf(-z, of_x[n][2 * r + i], v);
-                                total[m][n][2 * r + i] = fmaf(s, v, total[m][n][2 * r + i]);
-                            }
+                        for (int n = 0; n < kTilesN; ++n) {
+                            const float2 v = fma2(less2, make_float2(of_x[n][2 * r], of_x[n][2 * r + 1]),
+                                                  make_float2(acc[m][n][2 * r], acc[m][n][2 * r + 1]));
+                            total[m][n][r] = fma2(scale2, v, total[m][n][r]);
+                        }
                     }
             }
+        }
+    };
+    sm100::grid_wait();
+    Ring ring[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(ring[i], warp + i * kWarps);
+    for (uint32_t chunk = warp; chunk < chunks; chunk += kAhead * kWarps) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t at = chunk + i * kWarps;
+            if (at >= chunks) break;
+            consume(ring[i], at);
+            fetch(ring[i], at + kAhead * kWarps);
         }
     }
 #pragma unroll
@@ -184,8 +261,10 @@ __global__ void __launch_bounds__(kWarps * 32) qw_linear_w4_kernel(const Params 
 #pragma unroll
         for (int n = 0; n < kTilesN; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sums[warp][8 * n + 2 * t + (i & 1)][16 * m + 8 * (i >> 1) + g] = total[m][n][i];
+            for (int r = 0; r < 2; ++r) {
+                sums[warp][8 * n + 2 * t][16 * m + 8 * r + g] = total[m][n][r].x;
+                sums[warp][8 * n + 2 * t + 1][16 * m + 8 * r + g] = total[m][n][r].y;
+            }
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < kRows * kOutputs; e += kWarps * 32) {
         const uint32_t row = e / kOutputs, o = e - row * kOutputs;
@@ -193,23 +272,22 @@ __global__ void __launch_bounds__(kWarps * 32) qw_linear_w4_kernel(const Params 
         float v = p.bias ? widened(__ldg(p.bias + out0 + o)) : 0.0f;
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) v += sums[i][row][o];
-        p.y[(size_t)(row0 + row) * p.n + out0 + o] =
-            (uint16_t)(sm100::pack_bf16(v, 0.0f) & 0xffffu);
+        p.y[(size_t)(row0 + row) * p.n + out0 + o] = (uint16_t)(sm100::pack_bf16(v, 0.0f) & 0xffffu);
     }
 }
 
-template <int kTilesN, int kTilesM>
+template <int kWarps, int kTilesN, int kTilesM, int kAhead, int kCtas>
 int launch_tiles(const Params &p, cudaStream_t stream) {
     void (*kernel)(const Params);
     if (p.group >= kChunk)
-        kernel = p.zeros ? qw_linear_w4_kernel<kTilesN, kTilesM, 4, true>
-                         : qw_linear_w4_kernel<kTilesN, kTilesM, 4, false>;
+        kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 4, true, kAhead, kCtas>
+                         : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 4, false, kAhead, kCtas>;
     else if (p.group == 64)
-        kernel = p.zeros ? qw_linear_w4_kernel<kTilesN, kTilesM, 2, true>
-                         : qw_linear_w4_kernel<kTilesN, kTilesM, 2, false>;
+        kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 2, true, kAhead, kCtas>
+                         : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 2, false, kAhead, kCtas>;
     else
-        kernel = p.zeros ? qw_linear_w4_kernel<kTilesN, kTilesM, 1, true>
-                         : qw_linear_w4_kernel<kTilesN, kTilesM, 1, false>;
+        kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 1, true, kAhead, kCtas>
+                         : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 1, false, kAhead, kCtas>;
     const dim3 grid((p.n + 16 * kTilesM - 1) / (16 * kTilesM), (p.rows + 8 * kTilesN - 1) / (8 * kTilesN));
     return sm100::launch(kernel, grid, kWarps * 32, 0, 1, stream, p);
 }
@@ -233,7 +311,8 @@ extern "C" int qwcu_linear_w4_launch(const qwcu_linear_w4_args *a, int sm_count,
     p.k = a->k;
     p.n = a->n;
     p.group = a->group;
-    if (a->rows <= 8) return launch_tiles<1, 1>(p, stream);
-    if (a->rows <= 16) return launch_tiles<2, 1>(p, stream);
-    return launch_tiles<4, 2>(p, stream);
+    const uint32_t of_group = a->group / kChunk;
+    p.per_group = of_group > 1 ? (uint32_t)((0x100000000ull + of_group - 1) / of_group) : 0u;
+    if (a->rows <= 8) return launch_tiles<8, 1, 1, 2, 3>(p, stream);
+    return launch_tiles<4, 2, 2, 2, 3>(p, stream);
 }

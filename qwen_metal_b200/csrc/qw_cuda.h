@@ -303,9 +303,17 @@ typedef struct {
     const void *bias;   /* bf16 [n] or NULL */
     void *y;
     uint32_t rows, k, n, group;
+    uint32_t *status;
+    /* Bounded-wait exercise, as in qwcu_linear_args (the kernel for many rows only): the step of 128
+     * columns (>= 1, counted from a CTA's first) from which its producer loads nothing. */
+    long long wait_cycles;
+    uint32_t withhold_from;
 } qwcu_linear_w4_args;
 
+/* Few rows: the weights go through registers (cuda/qw_linear_w4.cu). */
 int qwcu_linear_w4_launch(const qwcu_linear_w4_args *args, int sm_count, qwcu_stream stream);
+/* Many rows: tcgen05 (cuda/qw_linear_w4_sm100.cu). */
+int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *args, int sm_count, qwcu_stream stream);
 
 /* Device properties needed by the host side. */
 int qwcu_device_sm_count(int device);

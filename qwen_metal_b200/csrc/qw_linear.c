@@ -142,6 +142,9 @@ int qw_gpu_qkv_norm_rope_bf16(h3_gpu *gpu, h3_gpu_tensor *query_out, h3_gpu_tens
     return launch_linear(gpu, &args, "Qwen QKV norm+rope");
 }
 
+/* Rows up to which 4-bit weights go through registers. */
+#define QW_W4_FEW_ROWS 16u
+
 /* NEW: output[rows, output_dim] = bf16(bias + input . w^T) with 4-bit weights, w = scale * (q - zero)
  * per group of columns. */
 int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
@@ -150,9 +153,9 @@ int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tenso
                           uint32_t input_dim, uint32_t output_dim, uint32_t group) {
     if (!gpu) return 0;
     if (!rows || !input_dim || !output_dim || !(group == 32 || group == 64 || (group && group % 128 == 0)) ||
-        input_dim % group || rows > (1u << 19)) {
+        input_dim % group || rows > (1u << 19) || input_dim > (1u << 22)) {
         qw_set_error(gpu, "4-bit linear: unsupported geometry (groups of 32, 64 or a multiple of 128 "
-                          "columns, whole groups, at most 2^19 rows)");
+                          "columns, whole groups, at most 2^19 rows and 2^22 columns)");
         return 0;
     }
     size_t input_count = (size_t)rows * input_dim, output_count = (size_t)rows * output_dim;
@@ -179,8 +182,10 @@ int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tenso
     if (!qw_bind(gpu)) return 0;
     qwcu_linear_w4_args args = {input->dev, weight->dev, scales->dev, zeros ? zeros->dev : NULL,
                                 bias ? bias->dev : NULL, output->dev, rows, input_dim, output_dim,
-                                group};
-    int rc = qwcu_linear_w4_launch(&args, qwcu_device_sm_count(gpu->device), gpu->stream);
+                                group, gpu->status_dev, gpu->linear_wait_cycles, gpu->linear_withhold[0]};
+    const int sms = qwcu_device_sm_count(gpu->device);
+    int rc = rows <= QW_W4_FEW_ROWS ? qwcu_linear_w4_launch(&args, sms, gpu->stream)
+                                    : qwcu_linear_w4_sm100_launch(&args, sms, gpu->stream);
     qw_count_launch(gpu, rc, "4-bit linear");
     return rc == 0;
 }

@@ -12,6 +12,8 @@ def make(rng, rows, inputs, outputs, group, with_zeros, with_bias):
     words = rng.integers(0, 2 ** 32, (outputs, inputs // 8), dtype=np.uint64).astype(np.uint32)
     scales = R.random_bf16(rng, outputs, inputs // group, std=0.02)
     zeros = R.random_bf16(rng, outputs, inputs // group, std=4.0) if with_zeros else None
+    if with_zeros == "whole":
+        zeros = abi.f32_to_bf16(rng.integers(0, 16, (outputs, inputs // group)).astype(np.float32))
     bias = R.random_bf16(rng, outputs) if with_bias else None
     return R.random_bf16(rng, rows, inputs), words, scales, zeros, bias
 
@@ -35,10 +37,11 @@ def linear(gpu, x, words, scales, zeros, bias, group, guard=64):
 SIZES = [(1, 32, 1, 32), (1, 128, 16, 128), (1, 4096, 6144, 128), (2, 192, 33, 64), (3, 2208, 100, 32),
          (5, 1024, 47, 256), (8, 384, 64, 128), (9, 160, 31, 32), (13, 4096, 513, 32), (16, 640, 129, 64),
          (17, 512, 95, 128), (32, 320, 65, 64), (33, 96, 40, 32), (64, 1408, 257, 128), (100, 2048, 130, 64),
-         (412, 1024, 384, 128), (300, 224, 77, 32)]
+         (412, 1024, 384, 128), (300, 224, 77, 32), (17, 4096, 128, 128), (48, 8192, 260, 512), (130, 4096, 200, 64),
+         (20, 2080, 1000, 32), (700, 512, 1290, 256)]
 
 
-@pytest.mark.parametrize("with_zeros,with_bias", [(False, False), (True, True)])
+@pytest.mark.parametrize("with_zeros,with_bias", [(False, False), (True, True), ("whole", False)])
 @pytest.mark.parametrize("rows,inputs,outputs,group", SIZES)
 def test_linear(gpu, rows, inputs, outputs, group, with_zeros, with_bias):
     rng = np.random.default_rng(rows * inputs + outputs)
@@ -118,3 +121,19 @@ def test_captured_and_twice_the_same(gpu, rows):
     gpu.lib.qw_gpu_graph_free(graph)
     for t in ts + [y]:
         gpu.free(t)
+
+
+@pytest.mark.parametrize("rows,inputs", [(100, 4096), (40, 512)])
+def test_bounded_waits_run_out_cleanly(gpu, rows, inputs):
+    """Steps from the second on stay away (nothing is in flight): the waits behind them run out, the submit
+    says so and the next call is right."""
+    rng = np.random.default_rng(10)
+    x, words, scales, _, _ = make(rng, rows, inputs, 300, 128, False, False)
+    gpu.check(gpu.lib.qw_gpu_debug_linear_waits(gpu.handle, 2_000_000, 1, 0))
+    try:
+        with pytest.raises(abi.GpuError, match="wait ran out"):
+            linear(gpu, x, words, scales, None, None, 128)
+    finally:
+        gpu.lib.qw_gpu_debug_linear_waits(gpu.handle, 0, 0, 0)
+    got = linear(gpu, x, words, scales, None, None, 128)
+    R.check_linear(got, *R.linear_w4(x, words, scales, None, None, 128))
