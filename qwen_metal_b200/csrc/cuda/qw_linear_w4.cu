@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) qw_linear_w4_kernel(const 
             const uint32_t at = chunk + i * kWarps;
             if (at >= chunks) break;
             consume(ring[i], at);
-            fetch(ring[i], at + kAhead * kWarps);
+            if (at + kAhead * kWarps < chunks) fetch(ring[i], at + kAhead * kWarps);
         }
     }
 #pragma unroll
