@@ -327,36 +327,80 @@ qw_paged_few_kernel(const Params p) {
             __syncthreads();
             if (last_one) {
                 __threadfence();
-                for (uint32_t r = warp; r < (uint32_t)kRows && row0 + r < rows; r += kWarps) {
+                // First the weights of all parts, a lane for each: loads behind a running maximum would
+                // wait for one another (55 parts: 25 us).  Then their sum; with fewer rows than warps,
+                // several warps share a row's parts.
+                const uint32_t parts = cta1 - cta0 + 1, here_rows = min((uint32_t)kRows, rows - row0);
+                float *weights = &merge_o[0][0][0];  // [row][part]
+                const auto part_of = [&](uint32_t c) {
+                    return p.partials + (size_t)(2 * (cta0 + c) + (c == 0)) * kPartial;
+                };
+                for (uint32_t r = warp; r < here_rows; r += kWarps) {
                     float top = -INFINITY, sum = 0.0f;
+                    for (uint32_t c = lane; c < parts; c += 32) {
+                        const float2 ml =
+                            __ldcg(reinterpret_cast<const float2 *>(part_of(c) + kMostRows * kDim) + r);
+                        weights[r * parts + c] = ml.x;
+                        const float m_new = fmaxf(top, ml.x), ref = m_new == -INFINITY ? 0.0f : m_new;
+                        sum = sum * fast_exp2(top - ref) + ml.y * fast_exp2(ml.x - ref);
+                        top = m_new;
+                    }
+                    float all = top;
+#pragma unroll
+                    for (int off = 1; off < 32; off <<= 1)
+                        all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, off));
+                    const float ref = all == -INFINITY ? 0.0f : all;
+                    sum *= fast_exp2(top - ref);
+#pragma unroll
+                    for (int off = 1; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    for (uint32_t c = lane; c < parts; c += 32)
+                        weights[r * parts + c] = fast_exp2(weights[r * parts + c] - ref);
+                    if (lane == 0) merge_l[0][r] = sum > 0.0f ? 1.0f / sum : 0.0f;
+                }
+                __syncthreads();
+                const uint32_t sharers = here_rows < (uint32_t)kWarps ? kWarps / here_rows : 1u;
+                float4 *shared_sums = reinterpret_cast<float4 *>(&merge_o[kWarps - 1][0][0]);  // [warp][lane]
+                for (uint32_t r0 = 0; r0 < here_rows; r0 += kWarps / sharers) {
+                    const uint32_t r = r0 + warp / sharers, share = warp % sharers;
+                    const bool mine = r < here_rows && warp / sharers < kWarps / sharers;
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    constexpr uint32_t kAhead = 8;
-                    for (uint32_t c = cta0; c <= cta1; c += kAhead) {
-                        float4 y[kAhead];
-                        float2 ml[kAhead];
+                    if (mine) {
+                        constexpr uint32_t kAhead = 8;
+                        for (uint32_t c = share; c < parts; c += kAhead * sharers) {
+                            float4 y[kAhead];
 #pragma unroll
-                        for (uint32_t i = 0; i < kAhead; ++i) {
-                            const uint32_t from = min(c + i, cta1);
-                            const float *other = p.partials + (size_t)(2 * from + (from == cta0)) * kPartial;
-                            y[i] = __ldcg(reinterpret_cast<const float4 *>(other + r * kDim) + lane);
-                            ml[i] = __ldcg(reinterpret_cast<const float2 *>(other + kMostRows * kDim) + r);
-                        }
+                            for (uint32_t i = 0; i < kAhead; ++i)
+                                y[i] = __ldcg(reinterpret_cast<const float4 *>(
+                                                  part_of(min(c + i * sharers, parts - 1)) + r * kDim) +
+                                              lane);
 #pragma unroll
-                        for (uint32_t i = 0; i < kAhead; ++i) {
-                            if (c + i > cta1) break;
-                            const float m_new = fmaxf(top, ml[i].x), ref = m_new == -INFINITY ? 0.0f : m_new;
-                            const float f = fast_exp2(top - ref), f_y = fast_exp2(ml[i].x - ref);
-                            sum = fmaf(sum, f, ml[i].y * f_y);
-                            x.x = fmaf(x.x, f, y[i].x * f_y), x.y = fmaf(x.y, f, y[i].y * f_y);
-                            x.z = fmaf(x.z, f, y[i].z * f_y), x.w = fmaf(x.w, f, y[i].w * f_y);
-                            top = m_new;
+                            for (uint32_t i = 0; i < kAhead; ++i) {
+                                const uint32_t from = c + i * sharers;
+                                const float f = from < parts ? weights[r * parts + from] : 0.0f;
+                                if (f == 0.0f) continue;
+                                x.x = fmaf(f, y[i].x, x.x), x.y = fmaf(f, y[i].y, x.y);
+                                x.z = fmaf(f, y[i].z, x.z), x.w = fmaf(f, y[i].w, x.w);
+                            }
                         }
                     }
-                    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-                    const uint32_t token = (row0 + r) / p.share, head = row0 + r - token * p.share;
-                    *reinterpret_cast<uint2 *>(
-                        p.out + ((size_t)(s.start + token) * p.heads + h * p.share + head) * kDim + 4 * lane) =
-                        make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+                    if (sharers > 1) {
+                        __syncthreads();  // (the weights have been read)
+                        shared_sums[tid] = x;
+                        __syncthreads();
+                        if (mine && share == 0)
+                            for (uint32_t i = 1; i < sharers; ++i) {
+                                const float4 y = shared_sums[tid + 32 * i];
+                                x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+                            }
+                    }
+                    if (mine && share == 0) {
+                        const float inv = merge_l[0][r];
+                        const uint32_t token = (row0 + r) / p.share, head = row0 + r - token * p.share;
+                        *reinterpret_cast<uint2 *>(p.out +
+                                                   ((size_t)(s.start + token) * p.heads + h * p.share + head) * kDim +
+                                                   4 * lane) =
+                            make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+                    }
                 }
             }
         }
