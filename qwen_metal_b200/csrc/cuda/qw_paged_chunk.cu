@@ -357,8 +357,9 @@ qw_paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         mbar_init_fence();
     }
     if (warp == kMmaWarp) tmem_alloc<1>(&ctl->tmem_base, kTmemCols);
-    grid_launch_dependents();
+    // In this order: the kernel for few rows may run beside this one, on what was there before both.
     grid_wait();
+    grid_launch_dependents();
     find_unit<kWarps>(p, blockIdx.x, extra->scan, &extra->unit);
     const Unit unit = extra->unit;
     paged::Sequence s = {0, 0, 0};
@@ -576,19 +577,15 @@ extern "C" size_t qwcu_paged_chunk_workspace_bytes(int sm_count) {
     return (size_t)sms_of(sm_count) * 2 * kTileM * (kHeadDim * sizeof(float) + sizeof(float2));
 }
 
-extern "C" int qwcu_paged_chunk_launch(const qwcu_paged_args *a, uint32_t least_rows, void *workspace,
-                                       int sm_count, qwcu_stream stream_, int *launched) {
-    *launched = 0;
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+namespace {
+
+// Everything but the tensor maps; 0 or a CUDA error.
+int make_params(const qwcu_paged_args *a, uint32_t least_rows, void *workspace, int sm_count, Params &p) {
     const uint32_t share = a->kv_heads ? a->heads / a->kv_heads : 0;
     if (!a->tokens || !a->cache.batch || !share || share > (uint32_t)kTileM || a->heads % a->kv_heads ||
-        a->cache.page_shift < 4 || !a->cache.pool_pages)
+        a->cache.page_shift < 4 || !a->cache.pool_pages ||
+        ((unsigned long long)a->cache.pool_pages << a->cache.page_shift) > 0x7fffffffull)
         return (int)cudaErrorInvalidValue;
-    const unsigned long long pool_rows = (unsigned long long)a->cache.pool_pages << a->cache.page_shift;
-    if (pool_rows > 0x7fffffffull) return (int)cudaErrorInvalidValue;
-    int rc = make_ready();
-    if (rc) return rc;
-    Params p;
     p.status = a->cache.status;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.wait_cycles = a->wait_cycles;
@@ -606,12 +603,27 @@ extern "C" int qwcu_paged_chunk_launch(const qwcu_paged_args *a, uint32_t least_
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + (size_t)p.sms * 2 * kTileM * kHeadDim);
     p.cache = {a->cache.page_table, a->cache.token_start, a->cache.cache_len, a->cache.batch, a->tokens,
                a->cache.table_width, a->cache.page_shift, a->cache.pool_pages, a->cache.status};
+    // A single sequence whose rows, if it has them all, give more units than half the SMs needs no
+    // second kernel.
+    const uint32_t unit_tokens = 2 * p.tile_tokens;
+    p.divide = p.sms > 1 && !(a->cache.batch == 1 && a->max_new >= a->tokens &&
+                              2ull * a->kv_heads * ((a->tokens + unit_tokens - 1) / unit_tokens) > p.sms);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int qwcu_paged_chunk_launch(const qwcu_paged_args *a, uint32_t least_rows, void *workspace,
+                                       int sm_count, qwcu_stream stream) {
+    Params p;
+    int rc = make_params(a, least_rows, workspace, sm_count, p);
+    if (rc || (rc = make_ready())) return rc;
     CUtensorMap map_q, map_k, map_v;
     const uint32_t box_rows = a->cache.page_shift < 7 ? 1u << a->cache.page_shift : (uint32_t)kTileN;
-    const uint32_t cols = a->kv_heads * kHeadDim;
-    if ((rc = make_query_map(&map_q, a->q, a->tokens, a->heads, share, p.tile_tokens))) return rc;
-    if ((rc = make_map_2d(&map_k, a->k_pages, (uint32_t)pool_rows, cols, box_rows))) return rc;
-    if ((rc = make_map_2d(&map_v, a->v_pages, (uint32_t)pool_rows, cols, box_rows))) return rc;
+    const uint32_t cols = a->kv_heads * kHeadDim, pool_rows = a->cache.pool_pages << a->cache.page_shift;
+    if ((rc = make_query_map(&map_q, a->q, a->tokens, a->heads, p.share, p.tile_tokens))) return rc;
+    if ((rc = make_map_2d(&map_k, a->k_pages, pool_rows, cols, box_rows))) return rc;
+    if ((rc = make_map_2d(&map_v, a->v_pages, pool_rows, cols, box_rows))) return rc;
     // As many CTAs as there can be units: a sequence's last block may be partly filled.
     const uint32_t unit_tokens = 2 * p.tile_tokens;
     const unsigned long long sequences = a->cache.batch < a->tokens ? a->cache.batch : a->tokens;
@@ -619,14 +631,18 @@ extern "C" int qwcu_paged_chunk_launch(const qwcu_paged_args *a, uint32_t least_
         (a->tokens / unit_tokens + sequences) * (unsigned long long)a->kv_heads;
     if (units > 0x3fffffffull) return (int)cudaErrorInvalidValue;
     const unsigned grid = units > p.sms ? (unsigned)units : p.sms;
-    // A single sequence whose rows, if it has them all, give more units than half the SMs needs no
-    // second kernel.
-    p.divide = !(a->cache.batch == 1 && a->max_new >= a->tokens &&
-                 2ull * a->kv_heads * ((a->tokens + unit_tokens - 1) / unit_tokens) > p.sms);
-    rc = launch(qw_paged_chunk_kernel, grid, kThreads, kSmem, 1, stream, map_q, map_k, map_v, p);
-    *launched = rc ? 0 : 1;
+    return launch(qw_paged_chunk_kernel, grid, kThreads, kSmem, 1, static_cast<cudaStream_t>(stream), map_q,
+                  map_k, map_v, p);
+}
+
+extern "C" int qwcu_paged_merge_launch(const qwcu_paged_args *a, uint32_t least_rows, void *workspace,
+                                       int sm_count, qwcu_stream stream, int *launched) {
+    Params p;
+    *launched = 0;
+    const int rc = make_params(a, least_rows, workspace, sm_count, p);
     if (rc || !p.divide) return rc;
-    rc = launch(qw_paged_merge_kernel, p.sms * kMergeSlices, kMergeWarps * 32, 0, 1, stream, p);
-    *launched = rc ? 1 : 2;
-    return rc;
+    *launched = 1;
+    // (units of two parts and more: at most one for every two SMs)
+    return launch(qw_paged_merge_kernel, p.sms / 2 * kMergeSlices, kMergeWarps * 32, 0, 1,
+                  static_cast<cudaStream_t>(stream), p);
 }

@@ -43,6 +43,7 @@ struct Params {
     uint16_t *out;
     uint32_t heads, kv_heads, share;  // share: query heads of a kv head
     uint32_t most_rows;               // sequences with more query rows are another kernel's
+    int beside;                       // that kernel is the one in front of this one in the stream
     float scale_log2;
     float *partials;     // two of each CTA
     uint32_t *counters;  // one of each CTA, zero between launches
@@ -96,8 +97,11 @@ qw_paged_few_kernel(const Params p) {
     __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
     __shared__ unsigned long long scan[kWarps], found_rest;
     __shared__ uint32_t found_b, last_one;
+    // The kernel for chunks starts this one when it has itself waited for all that was before it, and the two
+    // read and write nothing of each other's: this one waits for it only at its end, so that whoever waits for
+    // this one has waited for both.
     sm100::grid_launch_dependents();
-    sm100::grid_wait();
+    if (!p.beside) sm100::grid_wait();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
 
     // The tiles of every sequence, summed over the batch; a thread has a run of sequences.
@@ -127,7 +131,10 @@ qw_paged_few_kernel(const Params p) {
     const unsigned long long run = even > kLeast ? even : kLeast;
     unsigned long long at = run * blockIdx.x;
     const unsigned long long end = at + run < total ? at + run : total;
-    if (at >= total) return;
+    if (at >= total) {
+        if (p.beside) sm100::grid_wait();
+        return;
+    }
     if (at >= before && at < before + mine) {
         unsigned long long rest = at - before;
         for (uint32_t b = b_first;; ++b) {
@@ -408,6 +415,7 @@ qw_paged_few_kernel(const Params p) {
         at += count;
         rest += count;
     }
+    if (p.beside) sm100::grid_wait();
 }
 
 unsigned most_ctas(int sm_count) { return (unsigned)(sm_count > 0 ? sm_count : 148) * kCtasPerSm; }
@@ -419,8 +427,8 @@ extern "C" size_t qwcu_paged_few_workspace_bytes(int sm_count) {
     return ctas * 2 * kPartial * sizeof(float) + ctas * sizeof(uint32_t);
 }
 
-extern "C" int qwcu_paged_few_launch(const qwcu_paged_args *a, uint32_t most_rows, void *workspace,
-                                     int sm_count, qwcu_stream stream_) {
+extern "C" int qwcu_paged_few_launch(const qwcu_paged_args *a, uint32_t most_rows, int beside_chunks,
+                                     void *workspace, int sm_count, qwcu_stream stream_) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!a->tokens || !a->cache.batch || !a->heads || !a->kv_heads || a->heads % a->kv_heads ||
         a->cache.page_shift < 4 || !a->cache.pool_pages)
@@ -435,6 +443,7 @@ extern "C" int qwcu_paged_few_launch(const qwcu_paged_args *a, uint32_t most_row
     p.kv_heads = a->kv_heads;
     p.share = a->heads / a->kv_heads;
     p.most_rows = most_rows;
+    p.beside = beside_chunks;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.partials = static_cast<float *>(workspace);
     p.counters = reinterpret_cast<uint32_t *>(p.partials + (size_t)ctas * 2 * kPartial);

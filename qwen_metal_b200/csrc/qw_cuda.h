@@ -285,12 +285,16 @@ typedef struct {
  * registers (cuda/qw_paged_few.cu).  Workspaces are of one size for all calls on a device; this one
  * is zeroed when it is made. */
 size_t qwcu_paged_few_workspace_bytes(int sm_count);
-int qwcu_paged_few_launch(const qwcu_paged_args *args, uint32_t most_rows, void *workspace,
-                          int sm_count, qwcu_stream stream);
+int qwcu_paged_few_launch(const qwcu_paged_args *args, uint32_t most_rows, int beside_chunks,
+                          void *workspace, int sm_count, qwcu_stream stream);
 /* Sequences of at least least_rows query rows, heads / kv_heads <= 128: tcgen05
- * (cuda/qw_paged_chunk.cu), one or two kernels. */
+ * (cuda/qw_paged_chunk.cu), then the merge of units whose keys were divided over CTAs, if any can be.
+ * The kernel for few rows, launched between them with beside_chunks, runs on SMs that the chunks leave:
+ * it does not wait for the kernel in front of it until its end. */
 size_t qwcu_paged_chunk_workspace_bytes(int sm_count);
 int qwcu_paged_chunk_launch(const qwcu_paged_args *args, uint32_t least_rows, void *workspace,
+                            int sm_count, qwcu_stream stream);
+int qwcu_paged_merge_launch(const qwcu_paged_args *args, uint32_t least_rows, void *workspace,
                             int sm_count, qwcu_stream stream, int *launched);
 
 /* y[rows][n] = x[rows][k] . w[n][k]^T (+ bias), w = scale * (q - zero) with 4-bit q, eight to

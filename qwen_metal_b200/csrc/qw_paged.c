@@ -274,18 +274,21 @@ int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu
     /* Each kernel skips the other's sequences; one sequence alone needs no second kernel. */
     const uint32_t share = heads / kv_heads;
     const int chunks = share <= 128 && (uint64_t)max_new * share > QW_PAGED_FEW_ROWS;
+    const uint32_t least_rows = batch == 1 ? 0u : QW_PAGED_FEW_ROWS + 1u;
     int rc = 0;
     if (chunks) {
-        int launched;
-        rc = qwcu_paged_chunk_launch(&args, batch == 1 ? 0u : QW_PAGED_FEW_ROWS + 1u,
-                                     workspace + few_bytes, sms, gpu->stream, &launched);
-        for (; launched > (rc ? 0 : 1); launched--) qw_count_launch(gpu, 0, what);
+        rc = qwcu_paged_chunk_launch(&args, least_rows, workspace + few_bytes, sms, gpu->stream);
         qw_count_launch(gpu, rc, what);
     }
     if (!rc && (!chunks || batch > 1)) {
-        rc = qwcu_paged_few_launch(&args, chunks ? QW_PAGED_FEW_ROWS : UINT32_MAX, workspace, sms,
+        rc = qwcu_paged_few_launch(&args, chunks ? QW_PAGED_FEW_ROWS : UINT32_MAX, chunks, workspace, sms,
                                    gpu->stream);
         qw_count_launch(gpu, rc, what);
+    }
+    if (!rc && chunks) {
+        int launched;
+        rc = qwcu_paged_merge_launch(&args, least_rows, workspace + few_bytes, sms, gpu->stream, &launched);
+        if (rc || launched) qw_count_launch(gpu, rc, what);
     }
     return rc == 0;
 }
