@@ -116,6 +116,20 @@ __device__ __forceinline__ void find_unit(const Params &p, uint32_t index, unsig
     __syncthreads();
 }
 
+// The same for a batch of one sequence, by each thread for itself.  (A launch reads its code anew, line by line
+// from L2: what a CTA runs once in front of its first load costs more than its instructions.)
+__device__ __forceinline__ Unit unit_of_one(const Params &p, uint32_t index, const paged::Sequence &s) {
+    const uint32_t blocks = blocks_of(p, s), total = blocks * p.kv_heads;
+    Unit u;
+    u.b = 0;
+    u.parts = p.divide && total && total < p.sms ? p.sms / total : 1u;
+    const uint32_t at = index / u.parts;
+    u.active = at < total;
+    u.block = blocks - 1 - at / p.kv_heads;
+    u.h = at % p.kv_heads;
+    return u;
+}
+
 // What a unit has to do: its tokens and the key tiles that any of its rows sees.
 struct Plan {
     uint32_t token0;      // within the sequence
@@ -360,13 +374,19 @@ qw_paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     // In this order: the kernel for few rows may run beside this one, on what was there before both.
     grid_wait();
     grid_launch_dependents();
-    find_unit<kWarps>(p, blockIdx.x, extra->scan, &extra->unit);
-    const Unit unit = extra->unit;
+    Unit unit;
     paged::Sequence s = {0, 0, 0};
+    if (p.cache.batch == 1) {
+        s = paged::sequence(p.cache, 0);
+        unit = unit_of_one(p, blockIdx.x, s);
+    } else {
+        find_unit<kWarps>(p, blockIdx.x, extra->scan, &extra->unit);
+        unit = extra->unit;
+        if (unit.active) s = paged::sequence(p.cache, unit.b);
+    }
     Plan plan = {0, 0, 0, 0, false};
     int part = 0;
     if (unit.active) {
-        s = paged::sequence(p.cache, unit.b);
         plan = plan_of(p, unit, s);
         part = (int)(blockIdx.x % unit.parts);
     }
@@ -494,14 +514,25 @@ __global__ void __launch_bounds__(kMergeWarps * 32) qw_paged_merge_kernel(const 
     grid_wait();
     const uint32_t index = blockIdx.x / kMergeSlices, slice = blockIdx.x % kMergeSlices;
     // (unit `index` of a launch of at most sms CTAs: its first CTA)
-    find_unit<kMergeWarps>(p, 0, scan, &shared_unit);
-    const uint32_t parts_of_all = shared_unit.active ? shared_unit.parts : 1u;
-    __syncthreads();
-    if (parts_of_all == 1) return;
-    find_unit<kMergeWarps>(p, index * parts_of_all, scan, &shared_unit);
-    const Unit unit = shared_unit;
-    if (!unit.active) return;
-    const paged::Sequence s = paged::sequence(p.cache, unit.b);
+    Unit unit;
+    paged::Sequence s;
+    if (p.cache.batch == 1) {
+        s = paged::sequence(p.cache, 0);
+        unit = unit_of_one(p, 0, s);
+        if (!unit.active || unit.parts == 1) return;
+        unit = unit_of_one(p, index * unit.parts, s);
+        if (!unit.active) return;
+    } else {
+        find_unit<kMergeWarps>(p, 0, scan, &shared_unit);
+        if (!shared_unit.active || shared_unit.parts == 1) return;
+        const uint32_t at = index * shared_unit.parts;
+        __syncthreads();
+        find_unit<kMergeWarps>(p, at, scan, &shared_unit);
+        unit = shared_unit;
+        if (!unit.active) return;
+        s = paged::sequence(p.cache, unit.b);
+    }
+    const uint32_t parts_of_all = unit.parts;
     const Plan plan = plan_of(p, unit, s);
     if (plan.parts == 1) return;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;

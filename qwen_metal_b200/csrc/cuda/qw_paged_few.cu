@@ -83,7 +83,7 @@ template <int kRows>
 __device__ __forceinline__ Work work_of(const Params &p, const paged::Sequence &s) {
     const unsigned long long rows = (unsigned long long)s.fresh * p.share;
     Work w;
-    w.row_tiles = rows > p.most_rows ? 0u : (uint32_t)((rows + kRows - 1) / kRows);
+    w.row_tiles = rows > p.most_rows ? 0u : (uint32_t)((rows + kRows - 1) / kRows);  // (kRows: a power of two)
     w.tiles = max(1u, ((uint32_t)s.length + kKeys - 1) / kKeys);  // (no key: zeros are still written)
     return w;
 }
@@ -127,7 +127,10 @@ qw_paged_few_kernel(const Params p) {
         if (i < (int)warp) before += scan[i];
         total += scan[i];
     }
-    const unsigned long long even = (total + gridDim.x - 1) / gridDim.x;
+    // (Divisions in 32 bits where they are enough: a launch reads its code anew, line by line from L2, and one in
+    // 64 bits is long.)
+    const unsigned long long even =
+        total >> 31 ? (total + gridDim.x - 1) / gridDim.x : ((uint32_t)total + gridDim.x - 1) / gridDim.x;
     const unsigned long long run = even > kLeast ? even : kLeast;
     unsigned long long at = run * blockIdx.x;
     const unsigned long long end = at + run < total ? at + run : total;
@@ -162,7 +165,7 @@ qw_paged_few_kernel(const Params p) {
             ++b;
             continue;
         }
-        const uint32_t unit = (uint32_t)(rest / w.tiles), tile0 = (uint32_t)(rest - (unsigned long long)unit * w.tiles);
+        const uint32_t unit = rest >> 32 ? (uint32_t)(rest / w.tiles) : (uint32_t)rest / w.tiles, tile0 = (uint32_t)(rest - (unsigned long long)unit * w.tiles);
         const uint32_t h = unit / w.row_tiles, row0 = (unit - h * w.row_tiles) * kRows;
         const uint32_t count = (uint32_t)min((unsigned long long)(w.tiles - tile0), end - at);
         const uint32_t rows = (uint32_t)s.fresh * p.share;
@@ -293,7 +296,10 @@ qw_paged_few_kernel(const Params p) {
         // A unit that this CTA has from end to end is written out; a part goes to the workspace: the
         // CTA's second slot if the unit starts here, the first if it started in an earlier CTA.
         const unsigned long long unit_at = at - tile0;
-        const uint32_t cta0 = (uint32_t)(unit_at / run), cta1 = (uint32_t)((unit_at + w.tiles - 1) / run);
+        const unsigned long long unit_end = unit_at + w.tiles - 1;
+        const bool wide = (unit_end | run) >> 32;
+        const uint32_t cta0 = wide ? (uint32_t)(unit_at / run) : (uint32_t)unit_at / (uint32_t)run;
+        const uint32_t cta1 = wide ? (uint32_t)(unit_end / run) : (uint32_t)unit_end / (uint32_t)run;
         const bool whole = cta0 == cta1;
         float *part = p.partials + (size_t)(2 * blockIdx.x + (tile0 == 0)) * kPartial;
         for (uint32_t r = warp; r < (uint32_t)kRows && row0 + r < rows; r += kWarps) {
