@@ -51,6 +51,7 @@ struct Unit {
     uint32_t b, block, h;   // block: the rows' place in the sequence
     uint32_t parts;         // CTAs that share the launch's units, P of each
     int active;
+    int more;               // kSeveral: this CTA has another one
 };
 
 struct __align__(16) Extra {
@@ -70,7 +71,7 @@ __device__ __forceinline__ uint32_t blocks_of(const Params &p, const paged::Sequ
 
 // Unit of CTA `index` when every unit has P CTAs, with P so that all SMs have one; by all threads
 // of the CTA.  Units of a sequence stand together, its last blocks, which see the most keys, first.
-template <int kCtaWarps>
+template <int kCtaWarps, bool kSeveral>
 __device__ __forceinline__ void find_unit(const Params &p, uint32_t index, unsigned long long *scan,
                                           Unit *unit) {
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
@@ -97,6 +98,7 @@ __device__ __forceinline__ void find_unit(const Params &p, uint32_t index, unsig
     }
     const uint32_t parts = p.divide && total && total < p.sms ? p.sms / (uint32_t)total : 1u;
     const unsigned long long mine_unit = index / parts;
+    if (kSeveral && tid == 0) unit->more = mine_unit + gridDim.x < total;
     if (mine_unit >= before && mine_unit < before + mine) {
         unsigned long long rest = mine_unit - before;
         for (uint32_t b = first;; ++b) {
@@ -118,6 +120,7 @@ __device__ __forceinline__ void find_unit(const Params &p, uint32_t index, unsig
 
 // The same for a batch of one sequence, by each thread for itself.  (A launch reads its code anew, line by line
 // from L2: what a CTA runs once in front of its first load costs more than its instructions.)
+template <bool kSeveral>
 __device__ __forceinline__ Unit unit_of_one(const Params &p, uint32_t index, const paged::Sequence &s) {
     const uint32_t blocks = blocks_of(p, s), total = blocks * p.kv_heads;
     Unit u;
@@ -125,6 +128,7 @@ __device__ __forceinline__ Unit unit_of_one(const Params &p, uint32_t index, con
     u.parts = p.divide && total && total < p.sms ? p.sms / total : 1u;
     const uint32_t at = index / u.parts;
     u.active = at < total;
+    u.more = kSeveral && at + gridDim.x < total;
     u.block = blocks - 1 - at / p.kv_heads;
     u.h = at % p.kv_heads;
     return u;
@@ -339,6 +343,26 @@ __device__ __forceinline__ void fix_warp(const Params &p, SharedControl *ctl, Ex
     if (lane == 0) mbar_arrive(&ctl->bars[kBarKvFull + slot]);
 }
 
+__device__ __forceinline__ void init_barriers(SharedControl *ctl, Extra *extra) {
+    for (int i = 0; i < 2; ++i) mbar_init(&ctl->bars[kBarQFull + i], 1);
+    for (int i = 0; i < kStages; ++i) {
+        mbar_init(&ctl->bars[kBarKvFull + i], 1);
+        mbar_init(&ctl->bars[kBarKvEmpty + i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+        mbar_init(&ctl->bars[kBarSFull + i], 1);
+        mbar_init(&ctl->bars[kBarPFirst + i], kTileM / 32);
+        mbar_init(&ctl->bars[kBarPFull + i], kTileM / 32);
+        mbar_init(&ctl->bars[kBarOFinal + i], 1);
+    }
+    mbar_init(&ctl->bars[kBarMerge], kTileM / 32);
+    mbar_init(&extra->fix, 1);
+    mbar_init_fence();
+}
+
+// kSeveral: there may be more units than CTAs, so that a CTA takes several; without it the code is 1 to 3 %
+// faster (2048 tokens over 16384 keys: 464 us and 470).
+template <bool kSeveral>
 __global__ void __launch_bounds__(kThreads, 1)
 qw_paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const Params p) {
@@ -353,151 +377,160 @@ qw_paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int warp = warp_index();
     const int lane = tid & 31;
     if (warp == kTmaWarp && lane == 0) {
-        for (int i = 0; i < 2; ++i) mbar_init(&ctl->bars[kBarQFull + i], 1);
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(&ctl->bars[kBarKvFull + i], 1);
-            mbar_init(&ctl->bars[kBarKvEmpty + i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&ctl->bars[kBarSFull + i], 1);
-            mbar_init(&ctl->bars[kBarPFirst + i], kTileM / 32);
-            mbar_init(&ctl->bars[kBarPFull + i], kTileM / 32);
-            mbar_init(&ctl->bars[kBarOFinal + i], 1);
-        }
-        mbar_init(&ctl->bars[kBarMerge], kTileM / 32);
-        mbar_init(&extra->fix, 1);
+        init_barriers(ctl, extra);
         ctl->abort_flag = 0;
         ctl->wait_cycles = p.wait_cycles > 0 ? p.wait_cycles : kWaitCycles;
-        mbar_init_fence();
     }
     if (warp == kMmaWarp) tmem_alloc<1>(&ctl->tmem_base, kTmemCols);
     // In this order: the kernel for few rows may run beside this one, on what was there before both.
     grid_wait();
     grid_launch_dependents();
-    Unit unit;
-    paged::Sequence s = {0, 0, 0};
-    if (p.cache.batch == 1) {
-        s = paged::sequence(p.cache, 0);
-        unit = unit_of_one(p, blockIdx.x, s);
-    } else {
-        find_unit<kWarps>(p, blockIdx.x, extra->scan, &extra->unit);
-        unit = extra->unit;
-        if (unit.active) s = paged::sequence(p.cache, unit.b);
-    }
-    Plan plan = {0, 0, 0, 0, false};
-    int part = 0;
-    if (unit.active) {
-        plan = plan_of(p, unit, s);
-        part = (int)(blockIdx.x % unit.parts);
-    }
-    const bool active = unit.active && part < plan.parts;  // the same in all threads
-    const int begin = active ? (int)((long long)plan.tiles * part / plan.parts) : 0;
-    const int end = active ? (int)((long long)plan.tiles * (part + 1) / plan.parts) : 0;
-    const bool split = plan.split;
-
-    int my_limit = 0, sub = 0, tid_in_group = 0;
-    uint32_t my_token0 = 0;
-    if (active) {
-        if (warp == kTmaWarp && lane == 0) {
-            for (int i = 0; i < (split ? 1 : 2); ++i) {
-                Mbar *bar = &ctl->bars[kBarQFull + i];
-                mbar_expect_tx(bar, p.tile_tokens * p.share * kHeadDim * 2);
-                uint8_t *dst = smem_q + (size_t)i * kTileBytes;
-                const int head = (int)(unit.h * p.share);
-                const int token = (int)(s.start + plan.token0 + (uint32_t)i * p.tile_tokens);
-                tma_load_3d(dst, &map_q, bar, 0, head, token);
-                tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, head, token);
-            }
-        }
-        if (tid < kSoftmaxThreads) {
-            sub = tid >> 7;
-            tid_in_group = tid & 127;
-            my_token0 = plan.token0 + (split ? 0u : (uint32_t)sub * p.tile_tokens);
-            uint32_t token;
-            const bool real = row_token(p, (uint32_t)tid_in_group, my_token0, (uint32_t)s.fresh, token);
-            // (A row of no token is computed like its neighbours and never stored.)
-            my_limit = real ? max(0, s.length - s.fresh + (int)token + 1) : 0x7fffffff;
-        }
-        if (tid < 2) {
-            // A sub-tile's last token sees the most.
-            const uint32_t first = split ? plan.token0 : plan.token0 + (uint32_t)tid * p.tile_tokens;
-            const uint32_t past = min(first + p.tile_tokens, (uint32_t)s.fresh);
-            const int tiles = min((max(0, s.length - s.fresh + (int)past) + kTileN - 1) / kTileN, end);
-            const int mine = max(0, tiles - begin);
-            // Tiles are numbered from the part's first.
-            ctl->skip_lo = 0;
-            ctl->skip_hi = begin;
-            if (!split) {
-                ctl->tile_first[tid] = 0;
-                ctl->tile_count[tid] = mine;
-            } else {
-                const int half = (mine + 1) / 2;
-                ctl->tile_first[tid] = tid ? half : 0;
-                ctl->tile_count[tid] = tid ? mine - half : half;
-            }
-        }
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-
-    if (active) {
-        if (tid < kSoftmaxThreads) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-            const uint32_t warp_row0 = (uint32_t)(tid_in_group >> 5) * 32u;
-            const uint32_t box = smem_u32(smem_q + (size_t)sub * kTileBytes) + warp_row0 * 128u;
-            const auto has_rows = []() __attribute__((always_inline)) { return true; };
-            const auto store = [&p, &s, &unit, &plan, box, warp_row0, tid_in_group, sub, my_token0, lane](
-                                   uint32_t tmem_own, uint32_t tmem_other, float w_own, float w_other,
-                                   float inv, float m_row, float l_row) __attribute__((always_inline)) {
-                if (plan.parts > 1) {
-                    const size_t row = (size_t)blockIdx.x * (2 * kTileM) + (uint32_t)sub * kTileM;
-                    p.part_ml[row + (uint32_t)tid_in_group] = make_float2(m_row, l_row);
-                    write_part(tmem_own, tmem_other, w_own, w_other, box,
-                               p.part_o + (row + warp_row0) * kHeadDim);
-                    return;
-                }
-                long long where[4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t r = warp_row0 + 8u * i + ((uint32_t)lane >> 2);
-                    uint32_t token;
-                    const bool real = row_token(p, r, my_token0, (uint32_t)s.fresh, token);
-                    where[i] = real ? (long long)(((size_t)(s.start + token) * p.heads +
-                                                   unit.h * p.share + r % p.share) *
-                                                  kHeadDim)
-                                    : -1ll;
-                }
-                write_tokens(tmem_own, tmem_other, w_own, w_other, inv, box, p.out,
-                             make_longlong2(where[0], where[1]), make_longlong2(where[2], where[3]));
-            };
-            softmax_role<false, true>(p, ctl, sub, tid_in_group, my_limit, 0, 0, split, 0.0f, has_rows,
-                                      store);
+    uint32_t index = blockIdx.x;
+    bool again;
+    do {
+        Unit unit;
+        paged::Sequence s = {0, 0, 0};
+        if (p.cache.batch == 1) {
+            s = paged::sequence(p.cache, 0);
+            unit = unit_of_one<kSeveral>(p, index, s);
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+            find_unit<kWarps, kSeveral>(p, index, extra->scan, &extra->unit);
+            unit = extra->unit;
+            if (unit.active) s = paged::sequence(p.cache, unit.b);
         }
-        if (tid < kSoftmaxThreads) {
-        } else if (warp == kMmaWarp) {
-            if (split) mma_role_split(p, ctl, smem_q, smem_kv);
-            else mma_role(p, ctl, smem_q, smem_kv);
-        } else if (warp == kTmaWarp) {
-            tma_warp(p, ctl, extra, smem_kv, &map_k, &map_v, unit, s.length, begin, split);
-            // The loads of Q must have landed as well.
-            if (lane == 0)
-                for (int i = 0; i < (split ? 1 : 2); ++i)
-                    mbar_drain(&ctl->bars[kBarQFull + i], 0, ctl->wait_cycles);
-        } else if (warp == kFixWarp) {
-            // The tile that holds the end, if it is one of this CTA's and the end is inside it.
-            const int visited =
-                split ? ctl->tile_count[0] + ctl->tile_count[1] : max(ctl->tile_count[0], ctl->tile_count[1]);
-            const int last = s.length / kTileN;
-            if (s.length % kTileN && last >= begin && last < begin + visited)
-                fix_warp(p, ctl, extra, smem_kv, s.length, visited);
+        Plan plan = {0, 0, 0, 0, false};
+        int part = 0;
+        if (unit.active) {
+            plan = plan_of(p, unit, s);
+            part = (int)(index % unit.parts);
         }
-    }
+        const bool active = unit.active && part < plan.parts;  // the same in all threads
+        const int begin = active ? (int)((long long)plan.tiles * part / plan.parts) : 0;
+        const int end = active ? (int)((long long)plan.tiles * (part + 1) / plan.parts) : 0;
+        const bool split = plan.split;
 
-    tc_fence_before();
-    __syncthreads();
+        int my_limit = 0, sub = 0, tid_in_group = 0;
+        uint32_t my_token0 = 0;
+        if (active) {
+            if (warp == kTmaWarp && lane == 0) {
+                for (int i = 0; i < (split ? 1 : 2); ++i) {
+                    Mbar *bar = &ctl->bars[kBarQFull + i];
+                    mbar_expect_tx(bar, p.tile_tokens * p.share * kHeadDim * 2);
+                    uint8_t *dst = smem_q + (size_t)i * kTileBytes;
+                    const int head = (int)(unit.h * p.share);
+                    const int token = (int)(s.start + plan.token0 + (uint32_t)i * p.tile_tokens);
+                    tma_load_3d(dst, &map_q, bar, 0, head, token);
+                    tma_load_3d(dst + kHalfTileBytes, &map_q, bar, 64, head, token);
+                }
+            }
+            if (tid < kSoftmaxThreads) {
+                sub = tid >> 7;
+                tid_in_group = tid & 127;
+                my_token0 = plan.token0 + (split ? 0u : (uint32_t)sub * p.tile_tokens);
+                uint32_t token;
+                const bool real = row_token(p, (uint32_t)tid_in_group, my_token0, (uint32_t)s.fresh, token);
+                // (A row of no token is computed like its neighbours and never stored.)
+                my_limit = real ? max(0, s.length - s.fresh + (int)token + 1) : 0x7fffffff;
+            }
+            if (tid < 2) {
+                // A sub-tile's last token sees the most.
+                const uint32_t first = split ? plan.token0 : plan.token0 + (uint32_t)tid * p.tile_tokens;
+                const uint32_t past = min(first + p.tile_tokens, (uint32_t)s.fresh);
+                const int tiles = min((max(0, s.length - s.fresh + (int)past) + kTileN - 1) / kTileN, end);
+                const int mine = max(0, tiles - begin);
+                // Tiles are numbered from the part's first.
+                ctl->skip_lo = 0;
+                ctl->skip_hi = begin;
+                if (!split) {
+                    ctl->tile_first[tid] = 0;
+                    ctl->tile_count[tid] = mine;
+                } else {
+                    const int half = (mine + 1) / 2;
+                    ctl->tile_first[tid] = tid ? half : 0;
+                    ctl->tile_count[tid] = tid ? mine - half : half;
+                }
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+
+        if (active) {
+            if (tid < kSoftmaxThreads) {
+                asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+                const uint32_t warp_row0 = (uint32_t)(tid_in_group >> 5) * 32u;
+                const uint32_t box = smem_u32(smem_q + (size_t)sub * kTileBytes) + warp_row0 * 128u;
+                const auto has_rows = []() __attribute__((always_inline)) { return true; };
+                const auto store = [&p, &s, &unit, &plan, index, box, warp_row0, tid_in_group, sub, my_token0,
+                                    lane](
+                                       uint32_t tmem_own, uint32_t tmem_other, float w_own, float w_other,
+                                       float inv, float m_row, float l_row) __attribute__((always_inline)) {
+                    if (plan.parts > 1) {
+                        const size_t row = (size_t)index * (2 * kTileM) + (uint32_t)sub * kTileM;
+                        p.part_ml[row + (uint32_t)tid_in_group] = make_float2(m_row, l_row);
+                        write_part(tmem_own, tmem_other, w_own, w_other, box,
+                                   p.part_o + (row + warp_row0) * kHeadDim);
+                        return;
+                    }
+                    long long where[4];
+    #pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t r = warp_row0 + 8u * i + ((uint32_t)lane >> 2);
+                        uint32_t token;
+                        const bool real = row_token(p, r, my_token0, (uint32_t)s.fresh, token);
+                        where[i] = real ? (long long)(((size_t)(s.start + token) * p.heads +
+                                                       unit.h * p.share + r % p.share) *
+                                                      kHeadDim)
+                                        : -1ll;
+                    }
+                    write_tokens(tmem_own, tmem_other, w_own, w_other, inv, box, p.out,
+                                 make_longlong2(where[0], where[1]), make_longlong2(where[2], where[3]));
+                };
+                softmax_role<false, true>(p, ctl, sub, tid_in_group, my_limit, 0, 0, split, 0.0f, has_rows,
+                                          store);
+                if (kSeveral && unit.more) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
+            } else {
+                asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+            }
+            if (tid < kSoftmaxThreads) {
+            } else if (warp == kMmaWarp) {
+                if (split) mma_role_split(p, ctl, smem_q, smem_kv);
+                else mma_role(p, ctl, smem_q, smem_kv);
+            } else if (warp == kTmaWarp) {
+                tma_warp(p, ctl, extra, smem_kv, &map_k, &map_v, unit, s.length, begin, split);
+                // The loads of Q must have landed as well.
+                if (lane == 0)
+                    for (int i = 0; i < (split ? 1 : 2); ++i)
+                        mbar_drain(&ctl->bars[kBarQFull + i], 0, ctl->wait_cycles);
+            } else if (warp == kFixWarp) {
+                // The tile that holds the end, if it is one of this CTA's and the end is inside it.
+                const int visited =
+                    split ? ctl->tile_count[0] + ctl->tile_count[1] : max(ctl->tile_count[0], ctl->tile_count[1]);
+                const int last = s.length / kTileN;
+                if (s.length % kTileN && last >= begin && last < begin + visited)
+                    fix_warp(p, ctl, extra, smem_kv, s.length, visited);
+            }
+            if (kSeveral && tid >= kSoftmaxThreads && unit.more) {
+                __syncwarp();
+                asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLaunchRegs));
+            }
+        }
+
+        if (kSeveral && unit.more) fence_async_shared();  // (the rows' staging is where the next Q lands)
+        tc_fence_before();
+        __syncthreads();
+        // The next unit, with everything as at the start.
+        again = kSeveral && unit.more && !ctl->abort_flag;
+        if (again) {
+            index += gridDim.x;
+            if (warp == kTmaWarp && lane == 0) {
+                for (int i = 0; i < kBarCount; ++i) mbar_inval(&ctl->bars[i]);
+                mbar_inval(&extra->fix);
+                init_barriers(ctl, extra);
+            }
+            tc_fence_after();
+        }
+    } while (again);
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc<1>(ctl->tmem_base, kTmemCols);
@@ -518,16 +551,16 @@ __global__ void __launch_bounds__(kMergeWarps * 32) qw_paged_merge_kernel(const 
     paged::Sequence s;
     if (p.cache.batch == 1) {
         s = paged::sequence(p.cache, 0);
-        unit = unit_of_one(p, 0, s);
+        unit = unit_of_one<false>(p, 0, s);
         if (!unit.active || unit.parts == 1) return;
-        unit = unit_of_one(p, index * unit.parts, s);
+        unit = unit_of_one<false>(p, index * unit.parts, s);
         if (!unit.active) return;
     } else {
-        find_unit<kMergeWarps>(p, 0, scan, &shared_unit);
+        find_unit<kMergeWarps, false>(p, 0, scan, &shared_unit);
         if (!shared_unit.active || shared_unit.parts == 1) return;
         const uint32_t at = index * shared_unit.parts;
         __syncthreads();
-        find_unit<kMergeWarps>(p, at, scan, &shared_unit);
+        find_unit<kMergeWarps, false>(p, at, scan, &shared_unit);
         unit = shared_unit;
         if (!unit.active) return;
         s = paged::sequence(p.cache, unit.b);
@@ -597,7 +630,9 @@ int make_ready() {
     if (code != cudaSuccess) return (int)code;
     const bool tracked = dev >= 0 && dev < 64;
     if (tracked && ready[dev]) return 0;
-    code = cudaFuncSetAttribute(qw_paged_chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    for (const auto kernel : {qw_paged_chunk_kernel<false>, qw_paged_chunk_kernel<true>})
+        if (code == cudaSuccess)
+            code = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
     if (code == cudaSuccess && tracked) ready[dev] = true;
     return (int)code;
 }
@@ -655,14 +690,22 @@ extern "C" int qwcu_paged_chunk_launch(const qwcu_paged_args *a, uint32_t least_
     if ((rc = make_query_map(&map_q, a->q, a->tokens, a->heads, p.share, p.tile_tokens))) return rc;
     if ((rc = make_map_2d(&map_k, a->k_pages, pool_rows, cols, box_rows))) return rc;
     if ((rc = make_map_2d(&map_v, a->v_pages, pool_rows, cols, box_rows))) return rc;
-    // As many CTAs as there can be units: a sequence's last block may be partly filled.
-    const uint32_t unit_tokens = 2 * p.tile_tokens;
-    const unsigned long long sequences = a->cache.batch < a->tokens ? a->cache.batch : a->tokens;
-    const unsigned long long units =
-        (a->tokens / unit_tokens + sequences) * (unsigned long long)a->kv_heads;
-    if (units > 0x3fffffffull) return (int)cudaErrorInvalidValue;
-    const unsigned grid = units > p.sms ? (unsigned)units : p.sms;
-    return launch(qw_paged_chunk_kernel, grid, kThreads, kSmem, 1, static_cast<cudaStream_t>(stream), map_q,
+    // Units: full ones, and a last, partly filled block of each sequence that is not the other kernel's.
+    // Most sequences may well be that one's, and CTAs without a unit cost 2.5 us each: where their number
+    // could pass two of every SM, one of every SM is all there are, and CTAs with several units take them
+    // one after the other (255 single tokens over 200 keys beside a chunk of 128: 59.9 us, with a CTA for
+    // every unit there can be 77.6; 999 over 64 beside one of 32: 128 and 236).
+    const uint32_t unit_tokens = 2 * p.tile_tokens, least = (least_rows + p.share - 1) / p.share;
+    const uint32_t most = least ? a->tokens / least : a->tokens;
+    const unsigned long long sequences = a->cache.batch < most ? a->cache.batch : most;
+    const unsigned long long whole = (unsigned long long)(a->tokens / unit_tokens) * a->kv_heads;
+    const unsigned long long last = sequences * a->kv_heads;
+    if (whole + last > 0x3fffffffull) return (int)cudaErrorInvalidValue;
+    const bool several = last > 2 * p.sms;
+    const unsigned units = (unsigned)(whole + (several ? p.sms : last));
+    const unsigned grid = units > p.sms ? units : p.sms;
+    const auto kernel = several ? qw_paged_chunk_kernel<true> : qw_paged_chunk_kernel<false>;
+    return launch(kernel, grid, kThreads, kSmem, 1, static_cast<cudaStream_t>(stream), map_q,
                   map_k, map_v, p);
 }
 

@@ -67,6 +67,19 @@ def test_attention(gpu, new, length, page, heads, kv):
     check(cache, got, q)
 
 
+@pytest.mark.parametrize("new,heads,kv", [
+    ([5] * 200 + [1] * 300, 32, 8), ([33, 64, 65] * 25, 32, 8), ([20] * 60, 24, 24), ([1, 40] * 130, 8, 8)])
+def test_more_units_than_ctas(gpu, new, heads, kv):
+    """A CTA of the kernel for chunks takes several units, whole and divided in halves."""
+    rng = np.random.default_rng(len(new))
+    length = [n + int(x) for n, x in zip(new, rng.integers(0, 300, len(new)))]
+    cache = R.Cache(rng, new, length, 16, kv, tail=3)
+    q = R.random_bf16(rng, cache.tokens, heads, 128)
+    ok, error, got = attend(gpu, cache, q)
+    assert ok, error
+    check(cache, got, q)
+
+
 @pytest.mark.parametrize("max_new", [1, 3, 100, 5000])
 def test_max_new_only_chooses_kernels(gpu, max_new):
     rng = np.random.default_rng(2)
