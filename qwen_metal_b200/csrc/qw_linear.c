@@ -153,9 +153,9 @@ int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tenso
                           uint32_t input_dim, uint32_t output_dim, uint32_t group) {
     if (!gpu) return 0;
     if (!rows || !input_dim || !output_dim || !(group == 32 || group == 64 || (group && group % 128 == 0)) ||
-        input_dim % group || rows > (1u << 19) || input_dim > (1u << 22)) {
+        input_dim % group || rows > (1u << 19) || input_dim > (1u << 22) || output_dim > (1u << 30)) {
         qw_set_error(gpu, "4-bit linear: unsupported geometry (groups of 32, 64 or a multiple of 128 "
-                          "columns, whole groups, at most 2^19 rows and 2^22 columns)");
+                          "columns, whole groups, at most 2^19 rows, 2^22 columns and 2^30 outputs)");
         return 0;
     }
     size_t input_count = (size_t)rows * input_dim, output_count = (size_t)rows * output_dim;

@@ -216,7 +216,7 @@ def test_linear_refusals(fake):
     assert fake.says(name, dict(base, z=fake.bf16(20), b=fake.bf16(10))) == PASSED
     assert "h3_gpu_begin" in fake.says(name, base, open_chain=False)
     for change in (dict(rows=0), dict(input_dim=0), dict(output_dim=0), dict(group=0), dict(group=16), dict(group=96),
-                   dict(group=192), dict(input_dim=224), dict(rows=2 ** 19 + 1)):
+                   dict(group=192), dict(input_dim=224), dict(rows=2 ** 19 + 1), dict(output_dim=2 ** 30 + 1)):
         assert "unsupported" in fake.says(name, {**base, **change}), change
     for key, bad in dict(y=fake.bf16(29), x=fake.bf16(3 * 256 - 1), w=fake.u32(319), s=fake.bf16(19),
                          z=fake.bf16(19), b=fake.bf16(9)).items():
