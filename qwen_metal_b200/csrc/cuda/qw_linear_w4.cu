@@ -1,19 +1,41 @@
-// Linear layers with 4-bit weights: y = x W^T + bias, W[o][c] = s[o][g] (q[o][c] - z[o][g]), with a
-// scale s (and a zero point z, 8 where there is none) for every `group` columns.  HBM-bound on the
-// weights for few rows of x.
+// Linear layers with 4-bit weights for few rows of x: y = x W^T + bias, W[o][c] = s[o][g] (q[o][c] -
+// z[o][g]), with a scale s (and a zero point z, 8 where there is none) for every `group` columns.
 //
-// The weights are the M dimension of mma.sync (16 outputs x 16 columns), up to 32 rows of x its N
+// The weights are the M dimension of mma.sync (16 outputs x 16 columns), 8 or 16 rows of x its N
 // dimension: a warp reads 16 outputs' words straight into the fragments' registers, each word once,
 // with no shared memory between.  A product's sum does not depend on the order of the columns, so
 // the fragments take them as the words hold them: lane t of a quad has 32 neighbouring columns of
 // its output, and columns i and i + 4 of a word are one register (one shift and one and-or give
-// both as bf16 128 + q), which the x fragments match by two byte permutations.  q - 8 is exact in
-// bf16 and the group's sum is kept in fp32; scale and zero are applied to the sum:
-//   s (sum (q - 8) x - (z - 8) sum x), the second sum by an MMA with a matrix of ones.
-// So nothing is rounded before y is.
+// both as bf16 128 + q, exactly), which the x fragments match by two byte permutations.  A group's
+// sums are kept in fp32; scale and zero are applied to them:
+//   s (sum (128 + q) x - (128 + z) sum x), the second sum by an MMA with a matrix of ones.
+// So nothing is rounded before y is, and taking 128 away costs an fp32 sum 2^-24 of 136 |x|, where
+// a rounded weight would cost 2^-9 of its own.
 //
 // The warps of a CTA take the columns in turn, 128 at a time, and add their sums through shared
 // memory in a fixed order.
+//
+// What bounds it: the weights' bytes only in the limit.  One row through 4096 -> 32768 (67 MB, groups of
+// 128) takes 22 us, 3.1 TB/s; through 4096 -> 6144 (12.6 MB) 7 us: a launch reads its code and first
+// operands (4 us), then a warp has four or eight chunks to go.  13 rows take longer by loads of x from L2
+// and integer work that run beside the MMAs only in part.
+//
+// The shape of a CTA follows the tiles of 16 outputs that an SM gets, so that all are there at once and the
+// few columns a warp has left do not wait for few warps.  Passes of four layers of 4096 columns, groups of
+// 128 / 32, us (warps x tiles of outputs, CTAs that an SM must hold):
+//   up to 8 rows     2048 outputs   16x1 1  26.0 / 27.9    12x1 2  25.7 / 29.9     8x1 3  26.1 / 33.3
+//                    4096           12x1 2  26.5 / 32.6     8x1 3  27.2 / 38.8    16x1 1  30.5 / 42.0
+//                    6144            8x1 3  30.1 / 39.3     8x2 2  30.9 / 46.5    12x1 2  35.3 / 53.0
+//                    8192            8x2 2  31.0 / 47.2     8x1 3  40.9 / 64.2     4x1 4  35.0 / 56.0
+//                   12288            8x2 2  45.1 / 81.8     8x1 3  47.8 / 68.9
+//   9 to 16 rows     2048           16x1 1  24.4 / 28.2     8x1 1  27.7 / 36.7     4x2 3  40.9 / 62.3
+//                    4096            8x2 1  33.1 / 42.8     8x1 1  36.0 / 40.0     4x2 3  40.0 / 64.8
+//                    8192            6x2 2  44.2 / 61.8     4x2 3  54.1 / 77.0     8x2 1  55.2 / 73.5
+//                   12288            4x2 3  56.7 / 82.0     6x2 2  75.5 / 113      8x2 1  75.2 / 101
+// (12288 columns -> 4096, 13 rows: 8x2 1 66.5 / 109, 8x1 1 76.0 / 97.7, 4x2 3 99.2 / 209.)
+// The CTA's weights are asked for in L2 before the wait for the kernel in front: 12288 -> 4096, 16 rows,
+// groups of 64: 176 us, without 183.  x through shared memory and words through rings of cp.async were
+// slower than either (one row, 6144 outputs, eight layers: 53 us, with rings 71 to 90).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -23,7 +45,6 @@
 namespace {
 
 constexpr uint32_t kChunk = 128;  // columns of a warp's step
-
 
 struct Params {
     const uint16_t *x;
@@ -276,26 +297,27 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) qw_linear_w4_kernel(const 
     }
 }
 
-template <int kWarps, int kTilesN, int kTilesM, int kAhead, int kCtas>
-int launch_tiles(const Params &p, cudaStream_t stream) {
-    void (*kernel)(const Params);
-    if (p.group >= kChunk)
-        kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 4, true, kAhead, kCtas>
-                         : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 4, false, kAhead, kCtas>;
-    else if (p.group == 64)
-        kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 2, true, kAhead, kCtas>
-                         : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 2, false, kAhead, kCtas>;
-    else
-        kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 1, true, kAhead, kCtas>
-                         : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, 1, false, kAhead, kCtas>;
+template <int kWarps, int kTilesN, int kTilesM, int kFold, int kAhead, int kCtas>
+int launch_fold(const Params &p, cudaStream_t stream) {
+    const auto kernel = p.zeros ? qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, kFold, true, kAhead, kCtas>
+                                : qw_linear_w4_kernel<kWarps, kTilesN, kTilesM, kFold, false, kAhead, kCtas>;
     const dim3 grid((p.n + 16 * kTilesM - 1) / (16 * kTilesM), (p.rows + 8 * kTilesN - 1) / (8 * kTilesN));
     return sm100::launch(kernel, grid, kWarps * 32, 0, 1, stream, p);
+}
+template <int kWarps, int kTilesN, int kTilesM, int kAhead, int kCtas>
+int launch_narrow(const Params &p, cudaStream_t stream) {
+    return p.group == 64 ? launch_fold<kWarps, kTilesN, kTilesM, 2, kAhead, kCtas>(p, stream)
+                         : launch_fold<kWarps, kTilesN, kTilesM, 1, kAhead, kCtas>(p, stream);
+}
+template <int kWarps, int kTilesN, int kTilesM, int kAhead, int kCtas>
+int launch_tiles(const Params &p, cudaStream_t stream) {
+    return p.group >= kChunk ? launch_fold<kWarps, kTilesN, kTilesM, 4, kAhead, kCtas>(p, stream)
+                             : launch_narrow<kWarps, kTilesN, kTilesM, kAhead, kCtas>(p, stream);
 }
 
 }  // namespace
 
 extern "C" int qwcu_linear_w4_launch(const qwcu_linear_w4_args *a, int sm_count, qwcu_stream stream_) {
-    (void)sm_count;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const bool whole = a->group == 32 || a->group == 64 || (a->group && a->group % kChunk == 0);
     if (!a->rows || !a->n || !a->k || !whole || a->k % a->group) return (int)cudaErrorInvalidValue;
@@ -313,6 +335,18 @@ extern "C" int qwcu_linear_w4_launch(const qwcu_linear_w4_args *a, int sm_count,
     p.group = a->group;
     const uint32_t of_group = a->group / kChunk;
     p.per_group = of_group > 1 ? (uint32_t)((0x100000000ull + of_group - 1) / of_group) : 0u;
-    if (a->rows <= 8) return launch_tiles<8, 1, 1, 2, 3>(p, stream);
+    const unsigned tiles = a->n / 16 + (a->n % 16 != 0), sms = (unsigned)(sm_count > 0 ? sm_count : 148);
+    const bool wide = a->group >= kChunk;
+    if (a->rows <= 8) {
+        if (tiles <= sms) return launch_tiles<16, 1, 1, 2, 1>(p, stream);
+        if (tiles <= 2 * sms) return launch_tiles<12, 1, 1, 2, 2>(p, stream);
+        if (tiles <= 3 * sms) return launch_tiles<8, 1, 1, 2, 3>(p, stream);
+        if (wide || tiles <= 4 * sms) return launch_tiles<8, 1, 2, 2, 2>(p, stream);
+        return launch_narrow<8, 1, 1, 2, 3>(p, stream);
+    }
+    if (tiles <= sms) return launch_tiles<16, 2, 1, 2, 1>(p, stream);
+    if (tiles <= 2 * sms)
+        return wide ? launch_fold<8, 2, 2, 4, 2, 1>(p, stream) : launch_narrow<8, 2, 1, 2, 1>(p, stream);
+    if (tiles <= 4 * sms) return launch_tiles<6, 2, 2, 2, 2>(p, stream);
     return launch_tiles<4, 2, 2, 2, 3>(p, stream);
 }

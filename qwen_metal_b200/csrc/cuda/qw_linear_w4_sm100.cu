@@ -16,12 +16,15 @@
 //   1      MMA issuer, TMEM allocation
 //   4..7   weights: words -> bf16 -> TMEM
 //   8..11  totals: TMEM -> registers, then the result
-// A step of 128 columns takes about 1100 clocks with 112 rows of x, of which the tensor pipe needs 512: the
-// handing over between the roles takes the rest.  412 rows of 4096 x 4096, a pass: 41.0 us; with eight
-// warps for the weights 41.1, for weights and totals 43.2; with MMAs issued in a loop over their operands
-// 48.9; scales read when they are needed 52; one lane of a warp waiting for it 64.8.
+// What bounds it: a step of 128 columns takes about 1100 clocks with 112 rows of x, of which the tensor pipe
+// needs 512 (28 % active over a launch); the handing over between the roles takes the rest.  412 rows of
+// 4096 x 4096: 33 us, 420 TFLOP/s.  300 rows, a layer of a chain: groups of 128 columns 28.6 us, of 64, with
+// twice as many sums to be taken over, 40, of 32 69.  A pass of the 412 rows, begin to submit: 41.0 us; with
+// eight warps for the weights 41.1, for weights and totals 43.2; with MMAs issued in a loop over their
+// operands 48.9; one lane of a warp waiting for it 64.8.
 // A few tiles would leave SMs idle: up to eight CTAs of a cluster then take a share of the columns each
-// and add their totals through each other's shared memory, in the order of the CTAs.
+// and add their totals through each other's shared memory, in the order of the CTAs (30 rows of 4096 x 4096:
+// 10 us a layer).
 //
 // Every wait is bounded (status words, abort flag), and a CTA leaves no copy or MMA in flight.
 #include <cuda_bf16.h>
@@ -492,6 +495,34 @@ int launch_blocks(const Params &p, uint32_t group, const CUtensorMap &map_x, con
                          : launch_kernel<kBlocks, 1, false>(p, map_x, map_w, stream);
 }
 
+// Clusters of `size` CTAs that the device holds at once, asked for once.  (One CTA per SM: all variants have
+// the same threads, registers and, nearly, shared memory.)
+unsigned clusters_at_once(unsigned size) {
+    static unsigned known[64][9];
+    int dev = 0, count = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    const bool tracked = dev >= 0 && dev < 64;
+    if (tracked && known[dev][size]) return known[dev][size];
+    const auto kernel = qw_linear_w4_sm100_kernel<1, 1, false>;
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = size;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.gridDim = dim3(size);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kMostSmem;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&count, kernel, &config) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (tracked) known[dev][size] = (unsigned)count;
+    return (unsigned)count;
+}
+
 }  // namespace
 
 extern "C" int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *a, int sm_count, qwcu_stream stream_) {
@@ -515,19 +546,21 @@ extern "C" int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *a, int sm_
     // cause itself, gives up before those that wait behind it.)
     p.probes = 32 + (int)((a->wait_cycles > 0 ? a->wait_cycles : kWaitCycles) / kProbeCycles);
     p.withhold = a->withhold_from;
-    // Tiles of equal height, up to 128 rows; then as many CTAs to a tile's columns as the SMs have room
-    // for, of at least four steps each.
+    // Tiles of equal height, up to 128 rows; then as many CTAs to a tile's columns as there is room for, of at
+    // least four steps each.  Room is what the device says: clusters do not reach over its parts, so SMs are
+    // left over (24 rows of 4096, a pass of four layers: 2048 outputs are 16 clusters of eight, of which 14 fit:
+    // 55.2 us, with clusters of four 39.4; 4608 outputs are 36 of four, 70.9 us, of two 54.5).
     const uint32_t tiles = (a->rows + 127) / 128;
     p.tile_rows = ((a->rows + tiles - 1) / tiles + 15) / 16 * 16;
-    // As many stages as there is room for: with four, 412 rows of 4096 waited for the copies' latency.
+    // As many stages as there is room for, up to eight (412 rows of 4096: no difference between four and six).
     const uint32_t fit = (kMostSmem - 1024 - (uint32_t)sizeof(Control)) / (p.tile_rows * 256u + kWordBytes);
     p.stages = fit < (uint32_t)kMaxStages ? fit : (uint32_t)kMaxStages;
     p.idesc = instr_desc(kOutputs, p.tile_rows, false);
-    const unsigned sms = (unsigned)(sm_count > 0 ? sm_count : 148);
+    (void)sm_count;
     const uint32_t steps = (a->k + kChunk - 1) / kChunk;
     const unsigned long long ctas = (unsigned long long)((a->n + kOutputs - 1) / kOutputs) * tiles;
     p.splits = 1;
-    while (p.splits < 8 && ctas * p.splits * 2 <= sms && steps / (p.splits * 2) >= 4) p.splits *= 2;
+    while (p.splits < 8 && steps / (p.splits * 2) >= 4 && ctas <= clusters_at_once(p.splits * 2)) p.splits *= 2;
     CUtensorMap map_x, map_w;
     int rc;
     if ((rc = make_map_2d(&map_x, a->x, a->rows, a->k, p.tile_rows))) return rc;

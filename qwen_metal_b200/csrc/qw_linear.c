@@ -142,8 +142,15 @@ int qw_gpu_qkv_norm_rope_bf16(h3_gpu *gpu, h3_gpu_tensor *query_out, h3_gpu_tens
     return launch_linear(gpu, &args, "Qwen QKV norm+rope");
 }
 
-/* Rows up to which 4-bit weights go through registers. */
+/* Rows up to which 4-bit weights go through registers, and twice as many where the outputs are too few for
+ * all SMs otherwise.  Four layers of 4096 columns, groups of 128 / 32, there and on tcgen05, us: 16 rows to
+ * 4096 outputs 33 / 40 and 39 / 61, to 32768 153 / 246 and 149 / 311; 17 rows to 4096 52 / 65 and 40 / 58, to
+ * 1024 25 / 28 and 31 / 42. */
 #define QW_W4_FEW_ROWS 16u
+static int few_rows(uint32_t rows, uint32_t output_dim, int sms) {
+    return rows <= QW_W4_FEW_ROWS ||
+           (rows <= 2 * QW_W4_FEW_ROWS && 2 * (uint64_t)output_dim <= 16 * (uint64_t)sms);
+}
 
 /* NEW: output[rows, output_dim] = bf16(bias + input . w^T) with 4-bit weights, w = scale * (q - zero)
  * per group of columns. */
@@ -184,8 +191,8 @@ int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tenso
                                 bias ? bias->dev : NULL, output->dev, rows, input_dim, output_dim,
                                 group, gpu->status_dev, gpu->linear_wait_cycles, gpu->linear_withhold[0]};
     const int sms = qwcu_device_sm_count(gpu->device);
-    int rc = rows <= QW_W4_FEW_ROWS ? qwcu_linear_w4_launch(&args, sms, gpu->stream)
-                                    : qwcu_linear_w4_sm100_launch(&args, sms, gpu->stream);
+    int rc = few_rows(rows, output_dim, sms) ? qwcu_linear_w4_launch(&args, sms, gpu->stream)
+                                             : qwcu_linear_w4_sm100_launch(&args, sms, gpu->stream);
     qw_count_launch(gpu, rc, "4-bit linear");
     return rc == 0;
 }

@@ -222,7 +222,9 @@ static char *paged_workspace(h3_gpu *gpu, size_t few_bytes, size_t chunk_bytes) 
 }
 
 /* Query rows (new tokens x query heads of a kv head) up to which a sequence goes to the kernel for
- * few: one of its units. */
+ * few: one of its units.  With 8 instead of 16, 64 sequences of 4 tokens of 4 heads over 1000 keys take
+ * 110 us instead of 87 and 8 over 16000 keys 123 instead of 87; a mixed batch of 20 single tokens and 4
+ * chunks 121 instead of 126. */
 #define QW_PAGED_FEW_ROWS 16u
 
 int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,

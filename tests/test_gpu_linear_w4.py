@@ -38,7 +38,11 @@ SIZES = [(1, 32, 1, 32), (1, 128, 16, 128), (1, 4096, 6144, 128), (2, 192, 33, 6
          (5, 1024, 47, 256), (8, 384, 64, 128), (9, 160, 31, 32), (13, 4096, 513, 32), (16, 640, 129, 64),
          (17, 512, 95, 128), (32, 320, 65, 64), (33, 96, 40, 32), (64, 1408, 257, 128), (100, 2048, 130, 64),
          (412, 1024, 384, 128), (300, 224, 77, 32), (17, 4096, 128, 128), (48, 8192, 260, 512), (130, 4096, 200, 64),
-         (20, 2080, 1000, 32), (700, 512, 1290, 256)]
+         (20, 2080, 1000, 32), (700, 512, 1290, 256),
+         # each number of outputs for an SM that has a shape of its own
+         *[(rows, 640, outputs, group) for rows in (1, 8, 11) for outputs in (2001, 3100, 6000, 9001, 10100)
+           for group in (32, 64, 128)],
+         (17, 2176, 1500, 128), (20, 2080, 1300, 32), (32, 320, 1200, 64), (30, 1024, 1184, 128)]
 
 
 @pytest.mark.parametrize("with_zeros,with_bias", [(False, False), (True, True), ("whole", False)])
