@@ -16,8 +16,8 @@
 // memory in a fixed order.
 //
 // What bounds it: the weights' bytes only in the limit.  One row through 4096 -> 32768 (67 MB, groups of
-// 128) takes 22 us, 3.1 TB/s; through 4096 -> 6144 (12.6 MB) 7 us: a launch reads its code and first
-// operands (4 us), then a warp has four or eight chunks to go.  13 rows take longer by loads of x from L2
+// 128) takes 19 us in a chain of layers, 3.6 TB/s; through 4096 -> 6144 (12.6 MB) 5.5 us, 2.4 TB/s: a launch
+// reads its code and first operands (4 us), then a warp has four or eight chunks to go.  13 rows take longer by loads of x from L2
 // and integer work that run beside the MMAs only in part.
 //
 // The shape of a CTA follows the tiles of 16 outputs that an SM gets, so that all are there at once and the
