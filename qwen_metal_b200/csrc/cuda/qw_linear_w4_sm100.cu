@@ -43,21 +43,16 @@ constexpr uint32_t kChunk = 128;      // columns of a step
 constexpr int kMaxStages = 8;
 constexpr int kMostSmem = 227 * 1024;
 constexpr int kABuffers = 4;          // expanded weights of a step each, 64 columns of TMEM
-constexpr uint32_t kTmemCols = 512, kTmemA = 256, kTmemD = 128;  // sums at 0 and 128, weights from 256
+constexpr uint32_t kTmemCols = 512, kTmemA = 256;  // sums at 0, weights from 256
 constexpr int kWordBytes = kOutputs * 64;  // words of 128 outputs x 128 columns
-constexpr int kWeightWarp = 4, kTotalWarp = 8;  // first of four each
-// setmaxnreg redistributes what the CTA got at launch.
-constexpr int kTotalRegs = 216, kOtherRegs = 56, kLaunchRegs = 168;
-static_assert(128 * (kTotalRegs + kLaunchRegs + kOtherRegs) <= kThreads * kLaunchRegs, "registers");
+constexpr int kWeightWarp = 4;  // first of eight
 
 enum Barrier : int {
     kBarFull = 0,                        // x and words of a stage landed
-    kBarEmpty = kBarFull + kMaxStages,      // words taken (4 warps) and x consumed (MMA)
-    kBarAFull = kBarEmpty + kMaxStages,     // weights in TMEM (4 warps)
+    kBarEmpty = kBarFull + kMaxStages,   // words taken (8 warps) and x consumed (MMA)
+    kBarAFull = kBarEmpty + kMaxStages,  // weights in TMEM (8 warps)
     kBarAEmpty = kBarAFull + kABuffers,
-    kBarDFull = kBarAEmpty + kABuffers,  // 2: sums of a group complete
-    kBarDEmpty = kBarDFull + 2,          // 2: ... added (4 warps)
-    kBarDone = kBarDEmpty + 2,           // every MMA of the CTA is done
+    kBarDone = kBarAEmpty + kABuffers,   // every MMA of the CTA is done
     kBarCount = kBarDone + 1
 };
 
@@ -83,32 +78,40 @@ struct Params {
 };
 
 __device__ __forceinline__ float widened(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+                                     *reinterpret_cast<const __nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
     const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
                                      *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Scales or zero points of an output, a step ahead of their use: kUnits groups of a step, or one group
-// of several steps.
+// Scales or zero points of half a step's columns of an output, a step ahead of their use.  kUnits: groups of
+// a step (1: a group is a step or several).
 template <int kUnits>
 struct Ahead {
+    static constexpr uint32_t kHere = kUnits == 4 ? 2 : 1;
     const uint16_t *row;
-    uint32_t group, groups, left, steps;  // left: steps that the group has still to go
-    uint16_t next[kUnits];
-    __device__ __forceinline__ Ahead(const Params &p, const uint16_t *values, uint32_t output, uint32_t step)
-        : row(values + (size_t)output * p.groups), groups(p.groups), steps(p.group_steps) {
+    uint32_t group, last, left, steps;  // left: steps that the group has still to go
+    uint16_t next[kHere];
+    __device__ __forceinline__ Ahead(const Params &p, const uint16_t *values, uint32_t output, uint32_t step,
+                                     uint32_t half)
+        : row(values + (size_t)output * p.groups), last(p.groups - 1), steps(p.group_steps) {
         if constexpr (kUnits == 1) {
             group = step / steps;
             left = steps - (step - group * steps);
         } else {
-            group = step * kUnits;
+            group = step * kUnits + half * kHere;
         }
         read();
     }
+    // (Groups past the end are the last one's once more: their columns of x are zeros.)
     __device__ __forceinline__ void read() {
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) next[u] = __ldg(row + min(group + u, groups - 1));
+        for (uint32_t u = 0; u < kHere; ++u) next[u] = __ldg(row + min(group + u, last));
     }
     __device__ __forceinline__ void advance() {
         if constexpr (kUnits == 1) {
@@ -119,11 +122,6 @@ struct Ahead {
         read();
     }
 };
-// Groups of a step that lie within the columns.
-template <int kUnits>
-__device__ __forceinline__ uint32_t units_of(const Params &p, uint32_t step) {
-    return kUnits == 1 ? 1u : min((uint32_t)kUnits, p.groups - step * kUnits);
-}
 
 // Eight 4-bit columns of a word as four pairs of bf16 in their order, less the zero point.  0x4300 | q
 // is 128 + q; taking 128 away first leaves q, from which a zero of any value is taken with one rounding.
@@ -201,17 +199,14 @@ __device__ __forceinline__ T uniform(T v) {
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// The MMAs of a group of 16 * kCount columns, from column 16 * first on.  Unrolled, on operands in
-// uniform registers: in a loop over them an MMA took 150 clocks to issue, more than twice its execution.
-template <int kCount>
-__device__ __forceinline__ void issue_group(uint32_t d, uint32_t a, uint32_t x_lo, uint32_t box, uint32_t idesc,
-                                            int first) {
+// The MMAs of a step.  Unrolled, on operands in uniform registers: in a loop over them an MMA took 150 clocks
+// to issue, more than twice its execution.
+__device__ __forceinline__ void issue_step(uint32_t d, uint32_t a, uint32_t x_lo, uint32_t box, uint32_t idesc,
+                                           uint32_t accumulate) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-        const int kk = first + i;
-        mma_ts(d, a + (uint32_t)kk * 8u, x_lo + (uint32_t)(kk >> 2) * box + (uint32_t)(kk & 3) * 2u, idesc,
-               i > 0 ? 1u : 0u);
-    }
+    for (int i = 0; i < 8; ++i)
+        mma_ts(d, a + (uint32_t)i * 8u, x_lo + (uint32_t)(i >> 2) * box + (uint32_t)(i & 3) * 2u, idesc,
+               i > 0 ? 1u : accumulate);
 }
 
 __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
@@ -246,15 +241,11 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < kMaxStages; ++i) {
             mbar_init(&bars[kBarFull + i], 1);
-            mbar_init(&bars[kBarEmpty + i], 5);
+            mbar_init(&bars[kBarEmpty + i], 9);
         }
         for (int i = 0; i < kABuffers; ++i) {
-            mbar_init(&bars[kBarAFull + i], 4);
+            mbar_init(&bars[kBarAFull + i], 8);
             mbar_init(&bars[kBarAEmpty + i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars[kBarDFull + i], 1);
-            mbar_init(&bars[kBarDEmpty + i], 4);
         }
         mbar_init(&bars[kBarDone], 1);
         ctl->abort_flag = 0;
@@ -270,95 +261,72 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
     const Waiter w = {&ctl->abort_flag, p.status, p.wait_cycles > 0 ? p.wait_cycles : kWaitCycles};
     float *staged = reinterpret_cast<float *>(smem);  // the tile's totals [row of x][output], where the ring was
 
-    if (warp >= kTotalWarp) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTotalRegs));
-        float total[32 * kBlocks];
-#pragma unroll
-        for (int i = 0; i < 32 * kBlocks; ++i) total[i] = 0.0f;
-        const uint32_t row = (uint32_t)(warp - kTotalWarp) * 32 + lane, lanes = (uint32_t)(warp - kTotalWarp) * 32 << 16;
-        uint32_t d = 0;
-        bool ok = true;
-        Ahead<kUnits> scales(p, p.scales, min(out0 + row, p.n - 1), first);
-        for (uint32_t step = first; step < end && ok; ++step) {
-            const uint32_t units = units_of<kUnits>(p, step);
-            float now[kUnits];
-#pragma unroll
-            for (int u = 0; u < kUnits; ++u) now[u] = widened(scales.next[u]);
-            scales.advance();
-#pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                if ((uint32_t)u >= units) break;
-                const uint32_t buf = d & 1u;
-                const float scale = now[u];
-                ok = wait_in_line(w, &bars[kBarDFull + buf], (d >> 1) & 1u, (4u << 16) | (kBarDFull + buf), step);
-                if (!ok) break;
-                ++d;
-                tc_fence_after();
-#pragma unroll
-                for (int blk = 0; blk < kBlocks; ++blk) {
-                    uint32_t r[32];
-                    tmem_ld32(r, tmem + lanes + buf * kTmemD + blk * 32);
-                    tmem_wait_ld32(r);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        total[32 * blk + i] = fmaf(scale, __uint_as_float(r[i]), total[32 * blk + i]);
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[kBarDEmpty + buf]);
-            }
-        }
-        // When all MMAs are done, so are all loads and whoever reads them.
-        wait_in_line(w, &bars[kBarDone], 0, (4u << 16) | kBarDone, end);
-#pragma unroll
-        for (int i = 0; i < 32 * kBlocks; ++i)
-            if ((uint32_t)i < p.tile_rows) staged[i * kOutputs + row] = total[i];
-    } else if (warp >= kWeightWarp) {
-        const uint32_t row = (uint32_t)(warp - kWeightWarp) * 32 + lane, lanes = (uint32_t)(warp - kWeightWarp) * 32 << 16;
+    if (warp >= kWeightWarp) {
+        // A thread has half of a step's columns of an output.
+        const uint32_t half = (uint32_t)(warp - kWeightWarp) >> 2, row = (uint32_t)(warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
         uint32_t s = 0, phase = 0, t = 0;
+        bool ok = true;
+        const uint32_t output = min(out0 + row, p.n - 1);
+        Ahead<kUnits> scales(p, p.scales, output, first, half);
         // (without zero points the scales stand in for them, unused)
-        Ahead<kUnits> zeros(p, kZeros ? p.zeros : p.scales, min(out0 + row, p.n - 1), first);
+        Ahead<kUnits> zeros(p, kZeros ? p.zeros : p.scales, output, first, half);
         for (uint32_t step = first; step < end; ++step, ++t) {
             const uint32_t a = t % kABuffers;
-            uint32_t minus_zero[kUnits];
+            constexpr uint32_t kHere = Ahead<kUnits>::kHere;
+            uint32_t scale[kHere], minus_zero[kHere];
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) minus_zero[u] = kZeros ? (uint32_t)(zeros.next[u] ^ 0x8000u) * 0x10001u : 0u;
+            for (uint32_t u = 0; u < kHere; ++u) {
+                scale[u] = (uint32_t)scales.next[u] * 0x10001u;
+                minus_zero[u] = kZeros ? (uint32_t)(zeros.next[u] ^ 0x8000u) * 0x10001u : 0u;
+            }
+            scales.advance();
             if constexpr (kZeros) zeros.advance();
-            if (!wait_in_line(w, &bars[kBarFull + s], phase, (3u << 16) | (kBarFull + s), step)) break;
+            ok = wait_in_line(w, &bars[kBarFull + s], phase, (3u << 16) | (kBarFull + s), step);
+            if (!ok) break;
             // 64 bytes of an output, 16-byte pieces swizzled by the TMA over pairs of rows.
             const uint32_t words = smem_u32(smem + s * stage_bytes + 2 * box_bytes) + row * 64u;
-            uint4 v[4];
+            uint4 v[2];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) v[i] = ld_shared16(words + ((i ^ ((row >> 1) & 3u)) << 4));
+            for (uint32_t i = 0; i < 2; ++i) v[i] = ld_shared16(words + (((2 * half + i) ^ ((row >> 1) & 3u)) << 4));
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[kBarEmpty + s]);
             if (++s == p.stages) s = 0, phase ^= 1u;
-            if (!wait_in_line(w, &bars[kBarAEmpty + a], ((t / kABuffers) & 1u) ^ 1u, (3u << 16) | (kBarAEmpty + a),
-                                step))
-                break;
-            tc_fence_after();
+            uint32_t r[32];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t r[32];
+            for (int i = 0; i < 8; ++i) {
+                const uint4 &q = v[i >> 2];
+                const uint32_t word = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+                const uint32_t unit = kHere == 2 ? i >> 2 : 0;
+                uint32_t e[4];
+                expand<kZeros>(word, minus_zero[unit], e);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint4 &q = v[2 * half + (i >> 2)];
-                    const uint32_t word = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
-                    uint32_t zero = minus_zero[0];
-                    if constexpr (kUnits == 2) zero = minus_zero[half];
-                    if constexpr (kUnits == 4) zero = minus_zero[2 * half + (i >> 2)];
-                    uint32_t e[4];
-                    expand<kZeros>(word, zero, e);
-                    r[4 * i] = e[0], r[4 * i + 1] = e[1], r[4 * i + 2] = e[2], r[4 * i + 3] = e[3];
-                }
-                tmem_st32(tmem + lanes + kTmemA + a * 64 + half * 32, r);
+                for (int c = 0; c < 4; ++c) r[4 * i + c] = mul_bf16x2(e[c], scale[unit]);
             }
+            ok = wait_in_line(w, &bars[kBarAEmpty + a], ((t / kABuffers) & 1u) ^ 1u, (3u << 16) | (kBarAEmpty + a),
+                              step);
+            if (!ok) break;
+            tc_fence_after();
+            tmem_st32(tmem + lanes + kTmemA + a * 64 + half * 32, r);
             tmem_wait_st();
             tc_fence_before();
+            __syncwarp();
             if (lane == 0) mbar_arrive(&bars[kBarAFull + a]);
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        // When all MMAs are done, so are all loads and whoever reads them.
+        if (ok) ok = wait_in_line(w, &bars[kBarDone], 0, (3u << 16) | kBarDone, end);
+        tc_fence_after();
+#pragma unroll
+        for (int blk = 0; blk < kBlocks; ++blk) {
+            if ((blk & 1) != (int)half || !ok) continue;
+            uint32_t r[32];
+            tmem_ld32(r, tmem + lanes + blk * 32);
+            tmem_wait_ld32(r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if ((uint32_t)(32 * blk + i) < p.tile_rows)
+                    staged[(32 * blk + i) * kOutputs + row] = __uint_as_float(r[i]);
+        }
     }
     if (warp == 0) {
         uint32_t s = 0, phase = 0, t = 0;
@@ -383,7 +351,7 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
         }
     } else if (warp == 1) {
         bool ok = true;
-        uint32_t s = 0, t = 0, d = 0;
+        uint32_t s = 0, t = 0;
         const uint32_t d_tmem = uniform(tmem), x0 = uniform(smem_u32(smem) >> 4) | kDescKMajor;
         const uint32_t bar0 = uniform(smem_u32(bars)), box = box_bytes >> 4;
         const auto at = [&](uint32_t which) { return bar0 + which * (uint32_t)sizeof(Mbar); };
@@ -396,29 +364,13 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
                 break;
             }
             const uint32_t x_lo = x0 + s * (stage_bytes >> 4), a_tmem = d_tmem + kTmemA + a * 64;
-            const uint32_t units = units_of<kUnits>(p, step);
-#pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                if ((uint32_t)u >= units) break;
-                const uint32_t buf = d & 1u;
-                ok = probe(at(kBarDEmpty + buf), ((d >> 1) & 1u) ^ 1u, p.probes);
-                if (!ok) {
-                    gave_up(w, kBarDEmpty + buf, step);
-                    break;
-                }
-                ++d;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t to = d_tmem + buf * kTmemD;
-                    issue_group<8 / kUnits>(to, a_tmem, x_lo, box, p.idesc, 8 / kUnits * u);
-                    tc_commit<1>(at(kBarDFull + buf));
-                    if ((uint32_t)u + 1 == units) {
-                        tc_commit<1>(at(kBarEmpty + s));
-                        tc_commit<1>(at(kBarAEmpty + a));
-                    }
-                }
-                __syncwarp();
+            tc_fence_after();
+            if (elect_one()) {
+                issue_step(d_tmem, a_tmem, x_lo, box, p.idesc, t > 0 ? 1u : 0u);
+                tc_commit<1>(at(kBarEmpty + s));
+                tc_commit<1>(at(kBarAEmpty + a));
             }
+            __syncwarp();
             if (++s == p.stages) s = 0;
         }
         if (elect_one()) tc_commit<1>(&bars[kBarDone]);

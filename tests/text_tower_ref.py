@@ -111,14 +111,15 @@ def unpack(words):
 
 
 def linear_w4(x_bits, words, scales, zeros, bias, group):
-    """y in float64, the sum of magnitudes it is made of, and of those the part whose zeros are not whole."""
+    """y in float64, the sum of magnitudes it is made of, and those that roundings of weights go by."""
     q = unpack(words).astype(np.float64)
     z = np.full(scales.shape, 8.0) if zeros is None else wide(zeros)
     s, z = np.repeat(wide(scales), group, 1), np.repeat(z, group, 1)
     x = wide(x_bits)
     y = x @ (s * (q - z)).T
     size = np.abs(x) @ (np.abs(s) * (np.abs(q - 8) + np.abs(z - 8))).T
-    rounded = np.abs(x) @ np.where(z == np.rint(z), 0.0, np.abs(s * (q - z))).T
+    # with many rows a weight is rounded to bf16, and q - z before it where z is not whole
+    rounded = np.abs(x) @ (np.abs(s * (q - z)) * np.where(z == np.rint(z), 1.0, 2.0)).T
     if bias is not None:
         y, size = y + wide(bias), size + np.abs(wide(bias))
     return y, size, rounded
@@ -127,7 +128,7 @@ def linear_w4(x_bits, words, scales, zeros, bias, group):
 def check_linear(got_bits, y, size, rounded):
     # One rounding to bf16; sums of a group's 128 products (at most 4096 in one group) and of the groups
     # in fp32, each addition within 2^-23 of its operands: well below 2^-14 of the magnitudes for groups
-    # of up to 128 columns.  With more than 16 rows q - zero is rounded to bf16 where the zero is not whole.
+    # of up to 128 columns.  With more than 16 rows the weights are rounded to bf16, half a step each.
     err = np.abs(wide(got_bits) - y)
     bound = HALF_STEP * np.abs(y) + 2.0 ** -14 * size
     if got_bits.shape[0] > 16:
