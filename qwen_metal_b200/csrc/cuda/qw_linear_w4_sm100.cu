@@ -2,29 +2,26 @@
 //
 //   y = x W^T + bias, W[o][c] = s[o][g] (q[o][c] - z[o][g])
 //
-// The weights are the A operand, 128 outputs in the lanes of TMEM, and up to 128 rows of x the B
-// operand in shared memory.  A thread owns an output: it takes the words of 128 columns, makes q - z
-// in bf16 of them and stores them into TMEM, where the MMAs read A from; nothing of the expanded
-// weights goes through shared memory, whose bandwidth the MMAs need for B.  q - z is exact for whole z
-// of up to 8 bits (z = 8 without zero points) and rounded to bf16 otherwise, as a weight in bf16 would
-// be.  The scale is not in it: the products of a group of columns are summed by themselves, in fp32,
-// and a thread, which again owns an output, adds s times its sums to totals in registers while the next
-// group is multiplied.  With the scale in the weights they would all be rounded.
+// The weights are the A operand, 128 outputs in the lanes of TMEM, and up to 256 rows of x the B
+// operand in shared memory.  A thread owns half of an output's columns of a step: it takes their words, makes
+// s (q - z) in bf16 of them and stores them into TMEM, where the MMAs read A from; nothing of the expanded
+// weights goes through shared memory, whose bandwidth the MMAs need for B.  q - z is exact for whole z of up to
+// 8 bits (z = 8 without zero points) and rounded to bf16 otherwise; the weight is rounded once more, to half a
+// step, as it would be in a layer of bf16 weights.  All of a tile's products are summed in fp32 in TMEM.
 //
 // Warps (384 threads):
 //   0      TMA producer: 128 columns of x and of the weights' words a step
 //   1      MMA issuer, TMEM allocation
-//   4..7   weights: words -> bf16 -> TMEM
-//   8..11  totals: TMEM -> registers, then the result
-// What bounds it: a step of 128 columns takes about 1100 clocks with 112 rows of x, of which the tensor pipe
-// needs 512 (28 % active over a launch); the handing over between the roles takes the rest.  412 rows of
-// 4096 x 4096: 33 us, 420 TFLOP/s.  300 rows, a layer of a chain: groups of 128 columns 28.6 us, of 64, with
-// twice as many sums to be taken over, 40, of 32 69.  A pass of the 412 rows, begin to submit: 41.0 us; with
-// eight warps for the weights 41.1, for weights and totals 43.2; with MMAs issued in a loop over their
-// operands 48.9; one lane of a warp waiting for it 64.8.
+//   4..11  weights: words -> bf16 -> TMEM; at the end TMEM -> the result
+// What bounds it: for tiles of up to 128 rows the weights' integer work, a step of 128 columns about 1000 clocks
+// against 512 of MMA; a tile of 256 rows half hides it (4000 rows through 4096 x 12288: 337 us, 1.19 PFLOP/s).
+// 412 rows of 4096 x 4096: 30 us, begin to submit; 300 rows, a layer of a chain, 20 us.
+// With whole q - z as A and every group's sums taken out of TMEM and scaled in fp32 no weight is rounded, but
+// four warps do nothing else and every group is a hand-over: 4 layers of those 300 rows took 115 us (groups of
+// 128) and 278 us (of 32), as here 88 and 95; 4000 rows 574 and 1404 us, as here 423 and 441 (tiles of 128).
 // A few tiles would leave SMs idle: up to eight CTAs of a cluster then take a share of the columns each
-// and add their totals through each other's shared memory, in the order of the CTAs (30 rows of 4096 x 4096:
-// 10 us a layer).
+// and add their sums through each other's shared memory, in the order of the CTAs (30 rows of 4096 x 4096:
+// 8 us a layer).
 //
 // Every wait is bounded (status words, abort flag), and a CTA leaves no copy or MMA in flight.
 #include <cuda_bf16.h>
@@ -218,9 +215,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t cluster_addr) {
     return v;
 }
 
-// kBlocks: blocks of 32 rows of x in a tile (tile_rows may end inside the last).  kUnits: groups of a step
-// (1: a group is a step or several).
-template <int kBlocks, int kUnits, bool kZeros>
+// kUnits: groups of a step (1: a group is a step or several).
+template <int kUnits, bool kZeros>
 __global__ void __launch_bounds__(kThreads, 1)
 qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                           const Params p) {
@@ -316,16 +312,14 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
         // When all MMAs are done, so are all loads and whoever reads them.
         if (ok) ok = wait_in_line(w, &bars[kBarDone], 0, (3u << 16) | kBarDone, end);
         tc_fence_after();
-#pragma unroll
-        for (int blk = 0; blk < kBlocks; ++blk) {
-            if ((blk & 1) != (int)half || !ok) continue;
+#pragma unroll 1
+        for (uint32_t row0 = 32 * half; ok && row0 < p.tile_rows; row0 += 64) {
             uint32_t r[32];
-            tmem_ld32(r, tmem + lanes + blk * 32);
+            tmem_ld32(r, tmem + lanes + row0);
             tmem_wait_ld32(r);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if ((uint32_t)(32 * blk + i) < p.tile_rows)
-                    staged[(32 * blk + i) * kOutputs + row] = __uint_as_float(r[i]);
+            for (uint32_t i = 0; i < 32; ++i)
+                if (row0 + i < p.tile_rows) staged[(row0 + i) * kOutputs + row] = __uint_as_float(r[i]);
         }
     }
     if (warp == 0) {
@@ -417,11 +411,11 @@ int make_words_map(CUtensorMap *map, const void *base, uint32_t n, uint32_t word
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <int kBlocks, int kUnits, bool kZeros>
+template <int kUnits, bool kZeros>
 int launch_kernel(const Params &p, const CUtensorMap &map_x, const CUtensorMap &map_w, cudaStream_t stream) {
     // The opt-in to the shared memory is an attribute of the device: set on first use.
     static bool ready[64];
-    const auto kernel = qw_linear_w4_sm100_kernel<kBlocks, kUnits, kZeros>;
+    const auto kernel = qw_linear_w4_sm100_kernel<kUnits, kZeros>;
     int dev = 0;
     cudaError_t code = cudaGetDevice(&dev);
     if (code != cudaSuccess) return (int)code;
@@ -433,20 +427,9 @@ int launch_kernel(const Params &p, const CUtensorMap &map_x, const CUtensorMap &
     }
     const dim3 grid((p.n + kOutputs - 1) / kOutputs * p.splits, (p.rows + p.tile_rows - 1) / p.tile_rows);
     return launch(kernel, grid, kThreads,
-                  p.stages * (p.tile_rows * 256u + kWordBytes) + sizeof(Control) + 1024, (int)p.splits, stream, map_x, map_w, p);
+                  p.stages * (p.tile_rows * 256u + kWordBytes) + sizeof(Control) + 1024, (int)p.splits, stream,
+                  map_x, map_w, p);
 }
-template <int kBlocks>
-int launch_blocks(const Params &p, uint32_t group, const CUtensorMap &map_x, const CUtensorMap &map_w,
-                  cudaStream_t stream) {
-    if (p.zeros)
-        return group == 32   ? launch_kernel<kBlocks, 4, true>(p, map_x, map_w, stream)
-               : group == 64 ? launch_kernel<kBlocks, 2, true>(p, map_x, map_w, stream)
-                             : launch_kernel<kBlocks, 1, true>(p, map_x, map_w, stream);
-    return group == 32   ? launch_kernel<kBlocks, 4, false>(p, map_x, map_w, stream)
-           : group == 64 ? launch_kernel<kBlocks, 2, false>(p, map_x, map_w, stream)
-                         : launch_kernel<kBlocks, 1, false>(p, map_x, map_w, stream);
-}
-
 // Clusters of `size` CTAs that the device holds at once, asked for once.  (One CTA per SM: all variants have
 // the same threads, registers and, nearly, shared memory.)
 unsigned clusters_at_once(unsigned size) {
@@ -455,7 +438,7 @@ unsigned clusters_at_once(unsigned size) {
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
     const bool tracked = dev >= 0 && dev < 64;
     if (tracked && known[dev][size]) return known[dev][size];
-    const auto kernel = qw_linear_w4_sm100_kernel<1, 1, false>;
+    const auto kernel = qw_linear_w4_sm100_kernel<1, false>;
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -498,29 +481,43 @@ extern "C" int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *a, int sm_
     // cause itself, gives up before those that wait behind it.)
     p.probes = 32 + (int)((a->wait_cycles > 0 ? a->wait_cycles : kWaitCycles) / kProbeCycles);
     p.withhold = a->withhold_from;
-    // Tiles of equal height, up to 128 rows; then as many CTAs to a tile's columns as there is room for, of at
-    // least four steps each.  Room is what the device says: clusters do not reach over its parts, so SMs are
-    // left over (24 rows of 4096, a pass of four layers: 2048 outputs are 16 clusters of eight, of which 14 fit:
-    // 55.2 us, with clusters of four 39.4; 4608 outputs are 36 of four, 70.9 us, of two 54.5).
-    const uint32_t tiles = (a->rows + 127) / 128;
-    p.tile_rows = ((a->rows + tiles - 1) / tiles + 15) / 16 * 16;
+    // Tiles of equal height.  With 128 rows and less of a tile there may be few enough for several CTAs to a
+    // tile's columns, of at least four steps each.  Room is what the device says: clusters do not reach over
+    // its parts, so SMs are left over (24 rows of 4096, a pass of four layers: 2048 outputs are 16 clusters of
+    // eight, of which 14 fit: 55.2 us, with clusters of four 39.4; 4608 outputs are 36 of four, 70.9 us, of two
+    // 54.5).
+    const unsigned sms = (unsigned)(sm_count > 0 ? sm_count : 148);
+    const uint32_t steps = (a->k + kChunk - 1) / kChunk, low = (a->rows + 127) / 128;
+    const unsigned long long columns = (a->n + kOutputs - 1) / kOutputs;
+    const auto height = [&](uint32_t tiles) { return ((a->rows + tiles - 1) / tiles + 15) / 16 * 16; };
+    uint32_t tiles = low;
+    p.splits = 1;
+    while (p.splits < 8 && steps / (p.splits * 2) >= 4 && columns * tiles <= clusters_at_once(p.splits * 2))
+        p.splits *= 2;
+    // Otherwise as many tiles as make the waves cheapest, up to 256 rows each: a CTA's time goes as 170 + rows,
+    // of which the 170 are the weights.  4096 -> 4096, 500 rows: 21 us in tiles of 128, 26 of 256 (two CTAs
+    // each); 1000 rows, where 256 save the second wave, 40 and 29; 4000 rows to 12288 outputs 420 and 327.
+    if (p.splits == 1) {
+        const auto cost = [&](uint32_t count) {
+            return (columns * count + sms - 1) / sms * (170 + height(count));
+        };
+        for (uint32_t count = low - low / 2, step = 1 + low / 32; count < low; count += step)
+            if (columns * count * 2 > sms && cost(count) < cost(tiles)) tiles = count;
+    }
+    p.tile_rows = height(tiles);
     // As many stages as there is room for, up to eight (412 rows of 4096: no difference between four and six).
     const uint32_t fit = (kMostSmem - 1024 - (uint32_t)sizeof(Control)) / (p.tile_rows * 256u + kWordBytes);
     p.stages = fit < (uint32_t)kMaxStages ? fit : (uint32_t)kMaxStages;
     p.idesc = instr_desc(kOutputs, p.tile_rows, false);
-    (void)sm_count;
-    const uint32_t steps = (a->k + kChunk - 1) / kChunk;
-    const unsigned long long ctas = (unsigned long long)((a->n + kOutputs - 1) / kOutputs) * tiles;
-    p.splits = 1;
-    while (p.splits < 8 && steps / (p.splits * 2) >= 4 && ctas <= clusters_at_once(p.splits * 2)) p.splits *= 2;
     CUtensorMap map_x, map_w;
     int rc;
     if ((rc = make_map_2d(&map_x, a->x, a->rows, a->k, p.tile_rows))) return rc;
     if ((rc = make_words_map(&map_w, a->w, a->n, a->k / 8))) return rc;
-    switch ((p.tile_rows + 31) / 32) {
-        case 1: return launch_blocks<1>(p, a->group, map_x, map_w, stream);
-        case 2: return launch_blocks<2>(p, a->group, map_x, map_w, stream);
-        case 3: return launch_blocks<3>(p, a->group, map_x, map_w, stream);
-        default: return launch_blocks<4>(p, a->group, map_x, map_w, stream);
-    }
+    if (p.zeros)
+        return a->group == 32   ? launch_kernel<4, true>(p, map_x, map_w, stream)
+               : a->group == 64 ? launch_kernel<2, true>(p, map_x, map_w, stream)
+                                : launch_kernel<1, true>(p, map_x, map_w, stream);
+    return a->group == 32   ? launch_kernel<4, false>(p, map_x, map_w, stream)
+           : a->group == 64 ? launch_kernel<2, false>(p, map_x, map_w, stream)
+                            : launch_kernel<1, false>(p, map_x, map_w, stream);
 }

@@ -144,8 +144,8 @@ int qw_gpu_qkv_norm_rope_bf16(h3_gpu *gpu, h3_gpu_tensor *query_out, h3_gpu_tens
 
 /* Rows up to which 4-bit weights go through registers, and twice as many where the outputs are too few for
  * all SMs otherwise.  Four layers of 4096 columns, groups of 128 / 32, there and on tcgen05, us: 16 rows to
- * 4096 outputs 33 / 40 and 39 / 61, to 32768 153 / 246 and 149 / 311; 17 rows to 4096 52 / 65 and 40 / 58, to
- * 1024 25 / 28 and 31 / 42. */
+ * 4096 outputs 33 / 40 and 38 / 49, to 12288 60 / 82 and 76 / 112, to 32768 152 / 246 and 145 / 216; 24 rows to
+ * 4096 54 / 69 and 39 / 49, to 1024 25 / 28 and 31 / 37. */
 #define QW_W4_FEW_ROWS 16u
 static int few_rows(uint32_t rows, uint32_t output_dim, int sms) {
     return rows <= QW_W4_FEW_ROWS ||

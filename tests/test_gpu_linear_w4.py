@@ -42,6 +42,8 @@ SIZES = [(1, 32, 1, 32), (1, 128, 16, 128), (1, 4096, 6144, 128), (2, 192, 33, 6
          # each number of outputs for an SM that has a shape of its own
          *[(rows, 640, outputs, group) for rows in (1, 8, 11) for outputs in (2001, 3100, 6000, 9001, 10100)
            for group in (32, 64, 128)],
+         # tiles of more than 128 rows
+         (200, 512, 9600, 128), (140, 288, 12000, 32), (256, 192, 9600, 64), (1000, 640, 4100, 128), (257, 160, 18900, 32),
          (17, 2176, 1500, 128), (20, 2080, 1300, 32), (32, 320, 1200, 64), (30, 1024, 1184, 128)]
 
 
