@@ -17,12 +17,13 @@
 //
 // What bounds it: HBM, once there are some MB to read.  One sequence of 131072 keys (537 MB): 100 us,
 // 5.4 TB/s, 83 % of a plain copy's rate; 64 of up to 4096 keys 120 us (5.6 TB/s).  One of 2000 keys: 21 us
-// of which the chain's ends are 14; 1000 sequences of up to 64 keys 98 us, 3.5 times what their bytes take:
-// a unit of four tiles is a chain of four loads' latencies.  168 registers a thread keep a tile of K and V
+// of which the chain's ends are 14; 1000 sequences of up to 64 keys 58 us, twice what their bytes take:
+// a unit of four tiles is a chain of their loads' latencies.  168 registers a thread keep a tile of K and V
 // of each of 12 warps in flight.
 //
 // All key tiles of all units are numbered through and dealt out evenly, a run of them to a CTA,
-// whose warps take tiles in turn and merge at the end of a unit.  A unit that lies in several CTAs'
+// whose warps take tiles in turn and merge at the end of a unit, or, of several short units, a unit each.  A
+// unit that lies in several CTAs'
 // runs is merged by the last of them to finish, from partial results in the workspace in the order of
 // the CTAs, so that results do not depend on who is last.
 #include <cuda_runtime.h>
@@ -43,6 +44,10 @@ constexpr int kKeys = 16;         // keys of a tile; a page holds whole tiles
 // Tiles of a CTA: below, launch and merge cost more than they gain (8 sequences of 300 keys: 31.0 us, with
 // 4 tiles 31.8, 16 36.2, 24 41.7, 40 54.3).
 constexpr uint32_t kLeast = 8;
+// Tiles of the warps without a unit that a merge may cost.  Single tokens of 1000 sequences of up to 64 keys
+// 58.0 us, 256 of up to 200 49.7, of up to 1000 128; with 0 62.4, 53.5, 128; with 48 58.1, 51.4, 136; all
+// units merged 99.3, 58.4, 130, but 64 sequences of 4 tokens over up to 1000 keys 61.0 instead of 62.1.
+constexpr uint32_t kAlone = 16;
 constexpr int kMostRows = 16;     // query rows of a unit
 constexpr int kPartial = kMostRows * (kDim + 2);  // floats of a partial result: rows, then (m, l)
 
@@ -173,9 +178,20 @@ qw_paged_few_kernel(const Params p) {
             ++b;
             continue;
         }
-        const uint32_t unit = rest >> 32 ? (uint32_t)(rest / w.tiles) : (uint32_t)rest / w.tiles, tile0 = (uint32_t)(rest - (unsigned long long)unit * w.tiles);
+        uint32_t unit = rest >> 32 ? (uint32_t)(rest / w.tiles) : (uint32_t)rest / w.tiles;
+        const uint32_t tile0 = (uint32_t)(rest - (unsigned long long)unit * w.tiles);
+        const uint32_t left = (uint32_t)min(end - at, 0xffffffffull);
+        // Whole units that follow one another in a sequence: a warp takes one alone, which saves the merge
+        // (with fewer units than warps it must be worth the warps that have none).
+        uint32_t units = 1;
+        if (tile0 == 0 && w.tiles <= left / 2)
+            units = min(min((uint32_t)kWarps, left / w.tiles), w.row_tiles * p.kv_heads - unit);
+        const bool alone = units > 1 && w.tiles * (kWarps - units) <= kAlone;
+        if (alone) unit += min(warp, units - 1);
+        else units = 1;
         const uint32_t h = unit / w.row_tiles, row0 = (unit - h * w.row_tiles) * kRows;
-        const uint32_t count = (uint32_t)min((unsigned long long)(w.tiles - tile0), end - at);
+        const uint32_t count = alone ? (warp < units ? w.tiles : 0u) : min(w.tiles - tile0, left);
+        const uint32_t first = alone ? 0u : warp, stride = alone ? 1u : (uint32_t)kWarps;
         const uint32_t rows = (uint32_t)s.fresh * p.share;
         const int seen0 = s.length - s.fresh + 1;  // keys that the first token sees
 
@@ -217,8 +233,8 @@ qw_paged_few_kernel(const Params p) {
                     k[r][i] = load16(p.k_pages + pool + (g + 8 * r) * row_elements + 8 * t + 32 * i,
                                      (int)(key + g + 8 * r) < s.length);
         };
-        if (warp < count) load_k(tile0 + warp);
-        for (uint32_t i_tile = warp; i_tile < count; i_tile += kWarps) {
+        if (first < count) load_k(tile0 + first);
+        for (uint32_t i_tile = first; i_tile < count; i_tile += stride) {
             const int key0 = (int)((tile0 + i_tile) * kKeys);
             uint4 v[4][2];  // keys 2t, 2t + 1, 2t + 8, 2t + 9; dimensions 8g.. and 64 + 8g..
 #pragma unroll
@@ -237,7 +253,7 @@ qw_paged_few_kernel(const Params p) {
                     mma(sc[n], word(k[0][i >> 1], 2 * (i & 1)), word(k[1][i >> 1], 2 * (i & 1)),
                         word(k[0][i >> 1], 2 * (i & 1) + 1), word(k[1][i >> 1], 2 * (i & 1) + 1),
                         q[n][2 * i], q[n][2 * i + 1]);
-            if (i_tile + kWarps < count) load_k(tile0 + i_tile + kWarps);
+            if (i_tile + stride < count) load_k(tile0 + i_tile + stride);
 
             uint32_t pr[kTilesN][2];
 #pragma unroll
@@ -282,6 +298,34 @@ qw_paged_few_kernel(const Params p) {
             }
         }
 
+        if (alone) {
+            if (warp < units) {
+#pragma unroll
+                for (int n = 0; n < kTilesN; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float sum = l[n][i];
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                        const uint32_t r = row0 + 8 * n + 2 * t + i;
+                        if (r >= rows) continue;
+                        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                        const uint32_t token = r / p.share, head = r - token * p.share;
+                        uint16_t *to =
+                            p.out + ((size_t)(s.start + token) * p.heads + h * p.share + head) * kDim + 8 * g;
+#pragma unroll
+                        for (int d = 0; d < 2; ++d)
+                            *reinterpret_cast<uint4 *>(to + 64 * d) =
+                                make_uint4(pack_bf16(o[n][0][2 * d + i] * inv, o[n][1][2 * d + i] * inv),
+                                           pack_bf16(o[n][2][2 * d + i] * inv, o[n][3][2 * d + i] * inv),
+                                           pack_bf16(o[n][4][2 * d + i] * inv, o[n][5][2 * d + i] * inv),
+                                           pack_bf16(o[n][6][2 * d + i] * inv, o[n][7][2 * d + i] * inv));
+                    }
+            }
+            at += (unsigned long long)units * w.tiles;
+            rest += (unsigned long long)units * w.tiles;
+            continue;
+        }
         // The warps' results, merged by all threads.
 #pragma unroll
         for (int n = 0; n < kTilesN; ++n)

@@ -45,6 +45,11 @@ CASES = [
     ([1], [1], 16, 32, 8), ([1], [16], 16, 32, 8), ([1], [17], 16, 8, 1), ([1], [2000], 64, 32, 8),
     ([1, 1, 1], [5, 1000, 129], 16, 28, 4), ([1] * 9, list(range(1, 400, 45)), 32, 24, 24),
     ([1] * 150, [33 + i % 70 for i in range(150)], 16, 4, 2),
+    # many short ones: a warp for a unit
+    ([1] * 300, [i % 70 for i in range(300)], 16, 32, 8), ([1] * 400, [90 + i % 40 for i in range(400)], 64, 24, 24),
+    ([4] * 200, [4 + 3 * i % 60 for i in range(200)], 16, 32, 8),
+    ([1, 2, 3] * 100, [7 * i % 50 for i in range(300)], 32, 24, 24),
+    ([16] * 150, [16 + i for i in range(150)], 16, 5, 5),
     # a few
     ([2, 3, 1], [2, 77, 500], 16, 32, 8), ([4, 4], [300, 4], 128, 16, 2), ([5], [999], 256, 8, 8),
     ([7, 0, 2, 9], [40, 33, 2, 9], 16, 6, 2), ([1, 1], [0, 3], 16, 4, 4),
