@@ -22,10 +22,9 @@
 // of each of 12 warps in flight.
 //
 // All key tiles of all units are numbered through and dealt out evenly, a run of them to a CTA,
-// whose warps take tiles in turn and merge at the end of a unit, or, of several short units, a unit each.  A
-// unit that lies in several CTAs'
-// runs is merged by the last of them to finish, from partial results in the workspace in the order of
-// the CTAs, so that results do not depend on who is last.
+// whose warps take tiles in turn and merge at the end of a unit, or, of several short units, a unit
+// each.  A unit that lies in several CTAs' runs is merged by the last of them to finish, from partial
+// results in the workspace in the order of the CTAs, so that results do not depend on who is last.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
