@@ -39,6 +39,9 @@ constexpr int kOutputs = 128;         // of a tile: TMEM lanes
 constexpr uint32_t kChunk = 128;      // columns of a step
 constexpr int kMaxStages = 8;
 constexpr int kMostSmem = 227 * 1024;
+// More than half an SM's: a second CTA there would wait for the first one's TMEM, while that one may wait, by
+// its cluster or by the order of launches, for the second.
+constexpr size_t kLeastSmem = 116 * 1024;
 constexpr int kABuffers = 4;          // expanded weights of a step each, 64 columns of TMEM
 constexpr uint32_t kTmemCols = 512, kTmemA = 256;  // sums at 0, weights from 256
 constexpr int kWordBytes = kOutputs * 64;  // words of 128 outputs x 128 columns
@@ -426,12 +429,12 @@ int launch_kernel(const Params &p, const CUtensorMap &map_x, const CUtensorMap &
         if (tracked) ready[dev] = true;
     }
     const dim3 grid((p.n + kOutputs - 1) / kOutputs * p.splits, (p.rows + p.tile_rows - 1) / p.tile_rows);
-    return launch(kernel, grid, kThreads,
-                  p.stages * (p.tile_rows * 256u + kWordBytes) + sizeof(Control) + 1024, (int)p.splits, stream,
-                  map_x, map_w, p);
+    const size_t needed = p.stages * (p.tile_rows * 256u + kWordBytes) + sizeof(Control) + 1024;
+    return launch(kernel, grid, kThreads, needed > kLeastSmem ? needed : kLeastSmem, (int)p.splits, stream, map_x,
+                  map_w, p);
 }
-// Clusters of `size` CTAs that the device holds at once, asked for once.  (One CTA per SM: all variants have
-// the same threads, registers and, nearly, shared memory.)
+// Clusters of `size` CTAs that the device holds at once, asked for once.  (One CTA per SM, by its shared memory,
+// in all variants.)
 unsigned clusters_at_once(unsigned size) {
     static unsigned known[64][9];
     int dev = 0, count = 0;
