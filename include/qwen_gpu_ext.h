@@ -220,8 +220,9 @@ int qw_gpu_rotary_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_tensor *
  *                 neither read nor written
  *   cache_len     U32 [batch]: cache rows, the new tokens included; these are the last
  * All three are device tensors, so a step captured into a graph is replayed with other
- * lengths after writing them.  A page outside the pool, a token range outside the tensors
- * or a length beyond the page table is clamped and h3_gpu_submit returns 0 with the place.
+ * lengths after writing them.  For a page outside the pool, a token range outside the tensors
+ * or a length beyond the page table h3_gpu_submit returns 0 with the place: the tokens that it
+ * concerns are not appended, nor their queries rotated, and attention reads what does fit.
  * A sequence with more new tokens than cache rows has no row for the first of them: they
  * are not appended and attend to nothing.
  *

@@ -127,13 +127,14 @@ __global__ void __launch_bounds__(kThreads) qw_rotary_kernel(const Params p) {
     const uint32_t token0 = blockIdx.x * p.cta_tokens;
     const uint32_t count = min(p.cta_tokens, p.tokens - token0);
     if (p.into_cache) {
-        // Whose tokens they are: every thread looks at some sequences.
+        // Whose tokens they are: every thread looks at some sequences.  Tokens of one that does not fit its
+        // tensors have no row that can be told, and are left out like padding.
         if (threadIdx.x < kMaxTokens) sequence_of[threadIdx.x] = 0xffffffffu;
         __syncthreads();
         for (uint32_t b = threadIdx.x; b < p.cache.batch; b += kThreads) {
             const paged::Sequence s = paged::sequence(p.cache, b);
             for (uint32_t i = 0; i < count; ++i)
-                if (token0 + i - s.start < (uint32_t)s.fresh) sequence_of[i] = b;
+                if (s.fits && token0 + i - s.start < (uint32_t)s.fresh) sequence_of[i] = b;
         }
         __syncthreads();
         if (threadIdx.x < count) {
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) qw_rotary_kernel(const Params p) {
                 const paged::Sequence s = paged::sequence(p.cache, b);
                 const int row = s.length - s.fresh + (int)(token - s.start);
                 if (row >= 0) {
-                    at = (long long)paged::pool_row(p.cache, b, (uint32_t)row);
+                    at = paged::pool_row_or_none(p.cache, b, (uint32_t)row);
                     position = p.positions ? p.positions[token] : (uint32_t)row;
                 }
             }
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) qw_rotary_kernel(const Params p) {
     if (i >= count) return;
     const uint32_t lane = rest / p.slots, slot = rest - lane * p.slots;
     const long long row = p.into_cache ? row_of[i] : 0;
-    if (row < 0) return;  // padding behind the last sequence, or in front of the cache
+    if (row < 0) return;  // padding behind the last sequence, in front of the cache, or without a page
     const bool turn = slot * kVec < p.pairs;
     float c[kVec], s[kVec];
     // Where the two vectors lie in a head.
