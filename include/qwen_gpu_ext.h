@@ -242,7 +242,8 @@ int qw_gpu_rotary_append_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_t
 /* Attention of the new tokens over the cache, from single tokens to chunks of a prompt:
  * a token sees its sequence's cache rows up to its own.  query, output [tokens, heads, 128];
  * grouped heads as in qw_gpu_flash_sdpa_prefix_bf16; scale positive.  A token that sees
- * nothing stores zeros.  Cache rows past a sequence's end may hold anything; the values of
+ * nothing, or nothing but scores of minus infinity, stores zeros; NaN in its query or in a
+ * key that it sees makes its result NaN.  Cache rows past a sequence's end may hold anything; the values of
  * its new tokens must be finite where an earlier one's result is wanted.  max_new: new
  * tokens of the longest sequence, which only chooses the kernels (a sequence may have
  * more).  The first call makes a workspace of the context: run the op once before
