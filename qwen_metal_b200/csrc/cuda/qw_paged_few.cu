@@ -49,6 +49,11 @@ constexpr uint32_t kLeast = 8;
 constexpr uint32_t kAlone = 16;
 constexpr int kMostRows = 16;     // query rows of a unit
 constexpr int kPartial = kMostRows * (kDim + 2);  // floats of a partial result: rows, then (m, l)
+constexpr int kStride = kDim + 4;                 // floats of a row of a warp's result in shared memory
+// CTAs of a launch, so parts of a unit: their weights, a row after the other, take the place of the warps'
+// rows (176 SMs' CTAs; with one or two rows the last warp's place holds sums).
+constexpr unsigned kMostCtas = kWarps * kStride;
+static_assert(2 * kMostCtas <= (kWarps - 1) * 8 * kStride, "weights of two rows reach into the sums");
 
 struct Params {
     const uint16_t *q, *k_pages, *v_pages;
@@ -106,7 +111,6 @@ template <int kTilesN>
 __global__ void __launch_bounds__(kThreads, kTilesN == 1 ? kCtasPerSm : 2)
 qw_paged_few_kernel(const Params p) {
     constexpr int kRows = 8 * kTilesN;
-    constexpr int kStride = kDim + 4;
     __shared__ float merge_o[kWarps][kRows][kStride];
     __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
     __shared__ unsigned long long scan[kWarps], found_rest;
@@ -400,7 +404,7 @@ qw_paged_few_kernel(const Params p) {
                 // there a branch around one, behind which loads would wait for one another: four layers
                 // of one sequence of 8000 keys 78 us, with a branch 86, where it leaves the loop 108.
                 const uint32_t parts = cta1 - cta0 + 1, here_rows = min((uint32_t)kRows, rows - row0);
-                float *weights = &merge_o[0][0][0];  // [row][part]
+                float *weights = &merge_o[0][0][0];  // [row][part]: room for kMostCtas parts of every row
                 const auto part_of = [&](uint32_t c) {
                     return p.partials + (size_t)(2 * (cta0 + c) + (c == 0)) * kPartial;
                 };
@@ -480,7 +484,10 @@ qw_paged_few_kernel(const Params p) {
     if (p.beside) sm100::grid_wait();
 }
 
-unsigned most_ctas(int sm_count) { return (unsigned)(sm_count > 0 ? sm_count : 148) * kCtasPerSm; }
+unsigned most_ctas(int sm_count) {
+    const unsigned ctas = (unsigned)(sm_count > 0 ? sm_count : 148) * kCtasPerSm;
+    return ctas < kMostCtas ? ctas : kMostCtas;
+}
 
 }  // namespace
 
