@@ -261,10 +261,10 @@ int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu
  *   scales  bf16 [output_dim, input_dim / group]; zeros the same (any values), or NULL: 8
  *   bias    bf16 [output_dim] or NULL
  * group: 32, 64 or a multiple of 128, and input_dim whole groups; any output_dim up to
- * 2^30, up to 2^19 rows and 2^22 columns.  Sums are fp32.  Up to 16 rows (32 with few outputs),
- * inputs whose sums times 136 pass its range, or that are infinite, give NaN, and nothing but the
- * output is rounded; with more, the weights are rounded to bf16 first (q - zero too, where zeros
- * are not whole).  qw_w4_quantize_host makes such weights of bf16 ones. */
+ * 2^30, up to 2^19 rows and 2^22 columns.  Sums are fp32 and nothing but the output is rounded
+ * (zero points that are not whole: the weights within 3 * 2^-16 of themselves).  Infinite inputs
+ * give infinities or NaN; up to 16 rows (32 with few outputs) so do inputs whose sums times 136
+ * pass the range of fp32.  qw_w4_quantize_host makes such weights of bf16 ones. */
 int qw_gpu_linear_w4_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *input,
                           const h3_gpu_tensor *weight, const h3_gpu_tensor *scales,
                           const h3_gpu_tensor *zeros, const h3_gpu_tensor *bias, uint32_t rows,

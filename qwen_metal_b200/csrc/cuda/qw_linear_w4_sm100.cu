@@ -4,29 +4,35 @@
 //
 // The weights are the A operand, 128 outputs in the lanes of TMEM, and up to 256 rows of x the B
 // operand in shared memory.  A thread owns half of an output's columns of a step: it takes their words, makes
-// s (q - z) in bf16 of them and stores them into TMEM, where the MMAs read A from; nothing of the expanded
-// weights goes through shared memory, whose bandwidth the MMAs need for B.  q - z is exact for whole z of up to
-// 8 bits (z = 8 without zero points) and rounded to bf16 otherwise; the weight is rounded once more, to half a
-// step, as it would be in a layer of bf16 weights.  All of a tile's products are summed in fp32 in TMEM.
+// s (q - z) of them and stores them into TMEM, where the MMAs read A from; nothing of the expanded weights goes
+// through shared memory, whose bandwidth the MMAs need for B.  A weight is the sum of two bf16 numbers, and each
+// is an A operand of its own, so that no weight is rounded: s (q - 8) has 12 bits and is held whole, as is
+// s (q - z) for whole z; other zero points cost at most 3 * 2^-16 of the weight.  (One bf16 number, 2^-8 of the
+// weight off, is half of the MMAs, but a layer then answers otherwise than with few rows: 412 rows of 4096 x 4096
+// 28 us, begin to submit, as here 36; a sum of random weights' products 0.0022 of its size off and 0.0017, which
+// is the result's own rounding.)  All of a tile's products are summed in fp32 in TMEM.
 //
 // Warps (384 threads):
 //   0      TMA producer: 128 columns of x and of the weights' words a step
 //   1      MMA issuer, TMEM allocation
-//   4..11  weights: words -> bf16 -> TMEM; at the end TMEM -> the result
-// What bounds it: for tiles of up to 128 rows the weights' integer work, a step of 128 columns about 1000 clocks
-// against 512 of MMA; a tile of 256 rows half hides it (4000 rows through 4096 x 12288: 337 us, 1.19 PFLOP/s).
-// 412 rows of 4096 x 4096: 30 us, begin to submit; 300 rows, a layer of a chain, 20 us.
-// With whole q - z as A and every group's sums taken out of TMEM and scaled in fp32 no weight is rounded, but
-// four warps do nothing else and every group is a hand-over: 4 layers of those 300 rows took 115 us (groups of
-// 128) and 278 us (of 32), as here 88 and 95; 4000 rows 574 and 1404 us, as here 423 and 441 (tiles of 128).
+//   4..11  weights: words -> two parts in bf16 -> TMEM; at the end TMEM -> the result
+// What bounds it: the MMAs, 16 to a step of 128 columns.  Each takes some 30 clocks for its A out of TMEM and a
+// half for every row: a step of a 112-row tile 1500 clocks, of a 256-row tile 2800 (4000 rows through
+// 4096 x 12288: 590 us, 0.68 PFLOP/s of the layer, 1.36 of the MMAs).  412 rows of 4096 x 4096: 36 us, begin to
+// submit; 300 rows, a layer of a chain, 29 us.
+// With whole q - z as A and every group's sums taken out of TMEM and scaled in fp32 four warps do nothing else and
+// every group is a hand-over: 4 layers of those 300 rows took 115 us (groups of 128) and 278 us (of 32), as here
+// 121 and 126; 4000 rows 574 and 1404 us, as here 590 and 610; and a zero point that is not whole is rounded.
 // A few tiles would leave SMs idle: up to eight CTAs of a cluster then take a share of the columns each
 // and add their sums through each other's shared memory, in the order of the CTAs (30 rows of 4096 x 4096:
-// 8 us a layer).
+// 9 us a layer).
 //
 // Every wait is bounded (status words, abort flag), and a CTA leaves no copy or MMA in flight.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "qw_sm100.cuh"
 
@@ -42,8 +48,10 @@ constexpr int kMostSmem = 227 * 1024;
 // More than half an SM's: a second CTA there would wait for the first one's TMEM, while that one may wait, by
 // its cluster or by the order of launches, for the second.
 constexpr size_t kLeastSmem = 116 * 1024;
-constexpr int kABuffers = 4;          // expanded weights of a step each, 64 columns of TMEM
-constexpr uint32_t kTmemCols = 512, kTmemA = 256;  // sums at 0, weights from 256
+// TMEM: sums in the first 128 or 256 columns, behind them three or two buffers of a step's weights, 64 columns of
+// first parts and 64 of second ones.
+constexpr int kMaxABuffers = 3;
+constexpr uint32_t kTmemCols = 512, kACols = 128;
 constexpr int kWordBytes = kOutputs * 64;  // words of 128 outputs x 128 columns
 constexpr int kWeightWarp = 4;  // first of eight
 
@@ -51,8 +59,8 @@ enum Barrier : int {
     kBarFull = 0,                        // x and words of a stage landed
     kBarEmpty = kBarFull + kMaxStages,   // words taken (8 warps) and x consumed (MMA)
     kBarAFull = kBarEmpty + kMaxStages,  // weights in TMEM (8 warps)
-    kBarAEmpty = kBarAFull + kABuffers,
-    kBarDone = kBarAEmpty + kABuffers,   // every MMA of the CTA is done
+    kBarAEmpty = kBarAFull + kMaxABuffers,
+    kBarDone = kBarAEmpty + kMaxABuffers,  // every MMA of the CTA is done
     kBarCount = kBarDone + 1
 };
 
@@ -68,6 +76,7 @@ struct Params {
     uint32_t rows, k, n, groups;
     uint32_t tile_rows;    // rows of x of a tile, a multiple of 16: the MMA's N
     uint32_t idesc;
+    uint32_t tmem_a, a_buffers;  // where the weights' buffers begin, and how many there are
     uint32_t group_steps;  // steps of a group of 128 columns and more
     uint32_t stages;       // of the ring, at most kMaxStages
     uint32_t splits;       // CTAs of a cluster, over the columns
@@ -78,13 +87,19 @@ struct Params {
 };
 
 __device__ __forceinline__ float widened(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+    const __nv_bfloat162 v =
+        __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b),
+                *reinterpret_cast<const __nv_bfloat162 *>(&c));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+    const __nv_bfloat162 v = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162 *>(&a),
                                      *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+    const __nv_bfloat162 v = __hadd2_rn(*reinterpret_cast<const __nv_bfloat162 *>(&a),
                                      *reinterpret_cast<const __nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&v);
 }
@@ -123,19 +138,68 @@ struct Ahead {
     }
 };
 
-// Eight 4-bit columns of a word as four pairs of bf16 in their order, less the zero point.  0x4300 | q
-// is 128 + q; taking 128 away first leaves q, from which a zero of any value is taken with one rounding.
+constexpr uint32_t kSigns = 0x80008000u;
+
+// The two bf16 parts of a group's weights s (q - z), from v = 16 + q: `first` and `second` add up to a weight.
+//   without zero points   first = h (q - 8), second = l (q - 8) with h + l = s of four bits each: both have eight
+//                         bits at most, and (16 + q) h - 24 h is one instruction without a rounding.
+//   |z| <= 64             z = n + f, n whole: d = q - n is exact, and first = d s - c rounded, c the first part of
+//                         s f = c + e.  t = d s - first is exact: for d = 0 it is c; otherwise |first| is at least
+//                         half of s, so t, which is c but for half a step of `first`, is a multiple of 2^-8 (of
+//                         s's binade) below 1, or with |first| > 1 of 2^-7 below 2.  second = (t - c) - e: what
+//                         the rounding left, less the rest of s f, 2^-7 of the weight at most; its two roundings
+//                         cost 2^-16 and 2^-15 of the weight.
+//   any other             q - z as d and its error, by the two-sum of six additions that Knuth gives; first = d s
+//                         rounded, second what that left and the error's product.  (24 h may not overflow either.)
 template <bool kZeros>
-__device__ __forceinline__ void expand(uint32_t word, uint32_t minus_zero, uint32_t (&out)[4]) {
-    const uint32_t odd = word >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // columns 2i and 2i + 1: byte i of the word and of the shifted word
-        uint32_t v = __byte_perm(word, odd, 0x4400 + 0x1111 * i);
-        asm("lop3.b32 %0, %0, 0x000f000f, 0x43004300, 0xea;" : "+r"(v));
-        if constexpr (kZeros) out[i] = add_bf16x2(add_bf16x2(v, 0xc300c300u), minus_zero);
-        else out[i] = add_bf16x2(v, 0xc308c308u);
+struct Group {
+    uint32_t scale, minus_zero;  // bf16 pairs
+    uint32_t a, b, c, d;         // h, l, -24 h, -24 l; or -(16 + n), -c, -e
+    bool near;
+    __device__ __forceinline__ Group(uint16_t s, uint16_t z) {
+        scale = (uint32_t)s * 0x10001u;
+        if constexpr (kZeros) {
+            minus_zero = (uint32_t)(z ^ 0x8000u) * 0x10001u;
+            const float zero = widened(z), whole = rintf(zero), rest = widened(s) * (whole - zero);
+            near = fabsf(zero) <= 64.0f;
+            a = pack_bf16(-16.0f - whole, -16.0f - whole);
+            b = pack_bf16(rest, rest);
+            const float more = rest - __uint_as_float(b & 0xffff0000u);
+            c = pack_bf16(more, more);
+        } else {
+            minus_zero = 0xc100c100u;  // -8
+            near = (s & 0x7fffu) < 0x7b80u;  // 2^120
+            a = scale & 0xfff0fff0u;
+            b = add_bf16x2(scale, a ^ kSigns);
+            c = mul_bf16x2(a, 0xc1c0c1c0u);
+            d = mul_bf16x2(b, 0xc1c0c1c0u);
+        }
     }
-}
+    // Eight columns of a word as four pairs in their order.  0x4180 | q << 3 is 16 + q.
+    template <bool kNear>
+    __device__ __forceinline__ void expand(uint32_t word, uint32_t *first, uint32_t *second) const {
+        const uint32_t even = word << 3, odd = word >> 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // columns 2i and 2i + 1: the same byte of both
+            uint32_t v = __byte_perm(even, odd, 0x4400 + 0x1111 * i);
+            asm("lop3.b32 %0, %0, 0x00780078, 0x41804180, 0xea;" : "+r"(v));
+            if constexpr (!kNear) {
+                const uint32_t q = add_bf16x2(v, 0xc180c180u), sum = add_bf16x2(q, minus_zero);
+                const uint32_t y = add_bf16x2(sum, q ^ kSigns), x = add_bf16x2(sum, y ^ kSigns);
+                const uint32_t err = add_bf16x2(add_bf16x2(q, x ^ kSigns), add_bf16x2(minus_zero, y ^ kSigns));
+                first[i] = mul_bf16x2(sum, scale);
+                second[i] = fma_bf16x2(err, scale, fma_bf16x2(sum, scale, first[i] ^ kSigns));
+            } else if constexpr (kZeros) {
+                const uint32_t x = add_bf16x2(v, a);
+                first[i] = fma_bf16x2(x, scale, b);
+                second[i] = add_bf16x2(add_bf16x2(fma_bf16x2(x, scale, first[i] ^ kSigns), b), c);
+            } else {
+                first[i] = fma_bf16x2(v, a, c);
+                second[i] = fma_bf16x2(v, b, d);
+            }
+        }
+    }
+};
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
@@ -199,9 +263,9 @@ __device__ __forceinline__ T uniform(T v) {
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// The MMAs of a step.  Unrolled, on operands in uniform registers: in a loop over them an MMA took 150 clocks
+// The MMAs of half a step's A, 128 columns of one part.  Unrolled, on operands in uniform registers: in a loop over them an MMA took 150 clocks
 // to issue, more than twice its execution.
-__device__ __forceinline__ void issue_step(uint32_t d, uint32_t a, uint32_t x_lo, uint32_t box, uint32_t idesc,
+__device__ __forceinline__ void issue_part(uint32_t d, uint32_t a, uint32_t x_lo, uint32_t box, uint32_t idesc,
                                            uint32_t accumulate) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -242,7 +306,7 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
             mbar_init(&bars[kBarFull + i], 1);
             mbar_init(&bars[kBarEmpty + i], 9);
         }
-        for (int i = 0; i < kABuffers; ++i) {
+        for (int i = 0; i < kMaxABuffers; ++i) {
             mbar_init(&bars[kBarAFull + i], 8);
             mbar_init(&bars[kBarAEmpty + i], 1);
         }
@@ -264,21 +328,17 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
         // A thread has half of a step's columns of an output.
         const uint32_t half = (uint32_t)(warp - kWeightWarp) >> 2, row = (uint32_t)(warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
-        uint32_t s = 0, phase = 0, t = 0;
+        uint32_t s = 0, phase = 0, a = 0, a_phase = 1;
         bool ok = true;
         const uint32_t output = min(out0 + row, p.n - 1);
         Ahead<kUnits> scales(p, p.scales, output, first, half);
         // (without zero points the scales stand in for them, unused)
         Ahead<kUnits> zeros(p, kZeros ? p.zeros : p.scales, output, first, half);
-        for (uint32_t step = first; step < end; ++step, ++t) {
-            const uint32_t a = t % kABuffers;
+        for (uint32_t step = first; step < end; ++step) {
             constexpr uint32_t kHere = Ahead<kUnits>::kHere;
-            uint32_t scale[kHere], minus_zero[kHere];
-#pragma unroll
-            for (uint32_t u = 0; u < kHere; ++u) {
-                scale[u] = (uint32_t)scales.next[u] * 0x10001u;
-                minus_zero[u] = kZeros ? (uint32_t)(zeros.next[u] ^ 0x8000u) * 0x10001u : 0u;
-            }
+            // (where there is one, the second is not made)
+            const Group<kZeros> groups[2] = {{scales.next[0], zeros.next[0]},
+                                             {scales.next[kHere - 1], zeros.next[kHere - 1]}};
             scales.advance();
             if constexpr (kZeros) zeros.advance();
             ok = wait_in_line(w, &bars[kBarFull + s], phase, (3u << 16) | (kBarFull + s), step);
@@ -291,26 +351,29 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[kBarEmpty + s]);
             if (++s == p.stages) s = 0, phase ^= 1u;
-            uint32_t r[32];
+            uint32_t r[2][32];
+            const auto expand = [&](auto near) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint4 &q = v[i >> 2];
-                const uint32_t word = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
-                const uint32_t unit = kHere == 2 ? i >> 2 : 0;
-                uint32_t e[4];
-                expand<kZeros>(word, minus_zero[unit], e);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) r[4 * i + c] = mul_bf16x2(e[c], scale[unit]);
-            }
-            ok = wait_in_line(w, &bars[kBarAEmpty + a], ((t / kABuffers) & 1u) ^ 1u, (3u << 16) | (kBarAEmpty + a),
-                              step);
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 &q = v[i >> 2];
+                    const uint32_t word = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+                    groups[kHere == 2 ? i >> 2 : 0].template expand<decltype(near)::value>(word, r[0] + 4 * i,
+                                                                                          r[1] + 4 * i);
+                }
+            };
+            if (__all_sync(0xffffffffu, groups[0].near && groups[kHere - 1].near)) expand(std::true_type());
+            else expand(std::false_type());
+            ok = wait_in_line(w, &bars[kBarAEmpty + a], a_phase, (3u << 16) | (kBarAEmpty + a), step);
             if (!ok) break;
             tc_fence_after();
-            tmem_st32(tmem + lanes + kTmemA + a * 64 + half * 32, r);
+            const uint32_t to = tmem + lanes + p.tmem_a + a * kACols + half * 32;
+            tmem_st32(to, r[0]);
+            tmem_st32(to + kACols / 2, r[1]);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[kBarAFull + a]);
+            if (++a == p.a_buffers) a = 0, a_phase ^= 1u;
         }
         // When all MMAs are done, so are all loads and whoever reads them.
         if (ok) ok = wait_in_line(w, &bars[kBarDone], 0, (3u << 16) | kBarDone, end);
@@ -348,27 +411,28 @@ qw_linear_w4_sm100_kernel(const __grid_constant__ CUtensorMap map_x, const __gri
         }
     } else if (warp == 1) {
         bool ok = true;
-        uint32_t s = 0, t = 0;
+        uint32_t s = 0, a = 0, a_phase = 0;
         const uint32_t d_tmem = uniform(tmem), x0 = uniform(smem_u32(smem) >> 4) | kDescKMajor;
         const uint32_t bar0 = uniform(smem_u32(bars)), box = box_bytes >> 4;
         const auto at = [&](uint32_t which) { return bar0 + which * (uint32_t)sizeof(Mbar); };
-        for (uint32_t step = first; step < end && ok; ++step, ++t) {
-            const uint32_t a = t % kABuffers;
+        for (uint32_t step = first; step < end && ok; ++step) {
             // (The weights' warps have seen the stage: so has, through their arrivals, this one.)
-            ok = probe(at(kBarAFull + a), (t / kABuffers) & 1u, p.probes);
+            ok = probe(at(kBarAFull + a), a_phase, p.probes);
             if (!ok) {
                 gave_up(w, kBarAFull + a, step);
                 break;
             }
-            const uint32_t x_lo = x0 + s * (stage_bytes >> 4), a_tmem = d_tmem + kTmemA + a * 64;
+            const uint32_t x_lo = x0 + s * (stage_bytes >> 4), a_tmem = d_tmem + p.tmem_a + a * kACols;
             tc_fence_after();
             if (elect_one()) {
-                issue_step(d_tmem, a_tmem, x_lo, box, p.idesc, t > 0 ? 1u : 0u);
+                issue_part(d_tmem, a_tmem, x_lo, box, p.idesc, step > first ? 1u : 0u);
+                issue_part(d_tmem, a_tmem + kACols / 2, x_lo, box, p.idesc, 1u);
                 tc_commit<1>(at(kBarEmpty + s));
                 tc_commit<1>(at(kBarAEmpty + a));
             }
             __syncwarp();
             if (++s == p.stages) s = 0;
+            if (++a == p.a_buffers) a = 0, a_phase ^= 1u;
         }
         if (elect_one()) tc_commit<1>(&bars[kBarDone]);
         __syncwarp();
@@ -487,8 +551,8 @@ extern "C" int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *a, int sm_
     // Tiles of equal height.  With 128 rows and less of a tile there may be few enough for several CTAs to a
     // tile's columns, of at least four steps each.  Room is what the device says: clusters do not reach over
     // its parts, so SMs are left over (24 rows of 4096, a pass of four layers: 2048 outputs are 16 clusters of
-    // eight, of which 14 fit: 55.2 us, with clusters of four 39.4; 4608 outputs are 36 of four, 70.9 us, of two
-    // 54.5).
+    // eight, of which 14 fit: 58.2 us, with clusters of four 42.4; 4608 outputs are 36 of four, 74.6 us, of two
+    // 59.1).
     const unsigned sms = (unsigned)(sm_count > 0 ? sm_count : 148);
     const uint32_t steps = (a->k + kChunk - 1) / kChunk, low = (a->rows + 127) / 128;
     const unsigned long long columns = (a->n + kOutputs - 1) / kOutputs;
@@ -497,21 +561,25 @@ extern "C" int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *a, int sm_
     p.splits = 1;
     while (p.splits < 8 && steps / (p.splits * 2) >= 4 && columns * tiles <= clusters_at_once(p.splits * 2))
         p.splits *= 2;
-    // Otherwise as many tiles as make the waves cheapest, up to 256 rows each: a CTA's time goes as 170 + rows,
-    // of which the 170 are the weights.  4096 -> 4096, 500 rows: 21 us in tiles of 128, 26 of 256 (two CTAs
-    // each); 1000 rows, where 256 save the second wave, 40 and 29; 4000 rows to 12288 outputs 420 and 327.
+    // Otherwise as many tiles as make the waves cheapest, up to 256 rows each: a CTA's time goes as 60 + rows, with
+    // zero points 120 + rows, for which 90 + rows stands (60 or 170 there: 1 to 10 % slower or equal where it
+    // chooses otherwise).  A layer 4096 -> 4096, 500 rows: 32 us in tiles of 128, 50 of 256; 1000 rows, where 256
+    // save the second wave, 60 and 51; 4000 rows to 12288 outputs 685 and 593.
     if (p.splits == 1) {
         const auto cost = [&](uint32_t count) {
-            return (columns * count + sms - 1) / sms * (170 + height(count));
+            return (columns * count + sms - 1) / sms * (90 + height(count));
         };
         for (uint32_t count = low - low / 2, step = 1 + low / 32; count < low; count += step)
             if (columns * count * 2 > sms && cost(count) < cost(tiles)) tiles = count;
     }
     p.tile_rows = height(tiles);
-    // As many stages as there is room for, up to eight (412 rows of 4096: no difference between four and six).
+    // As many stages as there is room for, up to eight (412 rows of 4096, four layers: 123 us with
+    // six, 128 with four).
     const uint32_t fit = (kMostSmem - 1024 - (uint32_t)sizeof(Control)) / (p.tile_rows * 256u + kWordBytes);
     p.stages = fit < (uint32_t)kMaxStages ? fit : (uint32_t)kMaxStages;
     p.idesc = instr_desc(kOutputs, p.tile_rows, false);
+    p.tmem_a = p.tile_rows <= 128 ? 128 : 256;
+    p.a_buffers = (kTmemCols - p.tmem_a) / kACols;
     CUtensorMap map_x, map_w;
     int rc;
     if ((rc = make_map_2d(&map_x, a->x, a->rows, a->k, p.tile_rows))) return rc;

@@ -143,9 +143,11 @@ int qw_gpu_qkv_norm_rope_bf16(h3_gpu *gpu, h3_gpu_tensor *query_out, h3_gpu_tens
 }
 
 /* Rows up to which 4-bit weights go through registers, and twice as many where the outputs are too few for
- * all SMs otherwise.  Four layers of 4096 columns, groups of 128 / 32, there and on tcgen05, us: 16 rows to
- * 4096 outputs 33 / 40 and 38 / 49, to 12288 60 / 82 and 76 / 112, to 32768 152 / 246 and 145 / 216; 24 rows to
- * 4096 54 / 69 and 39 / 49, to 1024 25 / 28 and 31 / 37. */
+ * all SMs otherwise.  Four layers of 4096 columns, groups of 128 / of 32 with zero points, there and on tcgen05, us:
+ * 16 rows to 4096 outputs 33 / 41 and 42 / 54, to 12288 59 / 82 and 87 / 128, to 32768 153 / 244 and 164 / 242; 24 rows
+ * to 4096 54 / 70 and 42 / 54, to 1024 25 / 28 and 32 / 40.  12288 columns to 4096: 16 rows 67 / 96 and 77 / 110, 24
+ * rows 117 / 195 and 77 / 110; 1024 columns to 4096: 16 rows 20 / 21 and 32 / 38, but 24 rows 26 / 29 and 32 / 37, which
+ * the rule, by rows and outputs alone, leaves on tcgen05. */
 #define QW_W4_FEW_ROWS 16u
 static int few_rows(uint32_t rows, uint32_t output_dim, int sms) {
     return rows <= QW_W4_FEW_ROWS ||
