@@ -244,8 +244,8 @@ int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu
         qw_set_error(gpu, "%s: geometry too large", what);
         return 0;
     }
-    if (!(scale > 0.0f) || !isfinite(scale)) {
-        qw_set_error(gpu, "%s: the scale must be positive and finite", what);
+    if (!(scale > 0.0f) || !isfinite(scale * 1.4426950408889634f)) { /* (the kernels' exponents are powers of two) */
+        qw_set_error(gpu, "%s: the scale must be positive and, times log2(e), finite", what);
         return 0;
     }
     if (!require(gpu, query, count, H3_GPU_BF16, "paged attention query") ||
