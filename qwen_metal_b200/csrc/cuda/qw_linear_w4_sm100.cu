@@ -546,7 +546,8 @@ extern "C" int qwcu_linear_w4_sm100_launch(const qwcu_linear_w4_args *a, int sm_
     p.wait_cycles = a->wait_cycles;
     // (At least 32 probes; kProbeCycles is more than a probe takes, so that this role, which waits for the
     // cause itself, gives up before those that wait behind it.)
-    p.probes = 32 + (int)((a->wait_cycles > 0 ? a->wait_cycles : kWaitCycles) / kProbeCycles);
+    const long long budget = a->wait_cycles > 0 ? a->wait_cycles : kWaitCycles;
+    p.probes = 32 + (int)(budget / kProbeCycles < 1ll << 30 ? budget / kProbeCycles : 1ll << 30);
     p.withhold = a->withhold_from;
     // Tiles of equal height.  With 128 rows and less of a tile there may be few enough for several CTAs to a
     // tile's columns, of at least four steps each.  Room is what the device says: clusters do not reach over
