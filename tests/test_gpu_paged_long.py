@@ -36,3 +36,15 @@ def test_every_part_counts(gpu, new, length, heads, kv):
     R.check_attention(got[real], exact[real], size[real])
     again = attend(gpu, cache, q)
     assert (again[2] == got).all()
+
+
+@pytest.mark.parametrize("new,length,heads,kv", [([1], [700], 160, 1), ([3, 1], [90, 200], 130, 1), ([20], [150], 258, 2)])
+def test_more_heads_than_a_tile_of_rows(gpu, new, length, heads, kv):
+    """More than 128 query heads of a kv head: the kernel for few rows takes them all, whatever the tokens."""
+    rng = np.random.default_rng(heads)
+    cache = R.Cache(rng, new, length, 16, kv)
+    q = R.random_bf16(rng, cache.tokens, heads, 128)
+    ok, error, got = attend(gpu, cache, q)
+    assert ok, error
+    exact, size, real = R.attention(cache, q, SCALE)
+    R.check_attention(got[real], exact[real], size[real])
