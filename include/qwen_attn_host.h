@@ -51,7 +51,8 @@ uint32_t qw_rope_tables_blocks_host(const uint32_t *block_h, const uint32_t *blo
  * stretched for contexts `factor` times the trained length.  LINEAR: divided by factor.  THETA: theta
  * grown so that the slowest pair is divided by factor and the fastest kept.  PARTS: pairs that turn
  * more than 32 times within trained_length kept, those that turn less than once divided, the others
- * between; the magnitude is 0.1 ln(factor) + 1 (1 otherwise).  Returns 0 on arguments out of range. */
+ * between, linearly in their turns (a checkpoint whose ramp is over the pairs' index needs frequencies
+ * of its own); the magnitude is 0.1 ln(factor) + 1 (1 otherwise).  Returns 0 on arguments out of range. */
 enum {
     QW_ROTARY_SCALE_NONE = 0,
     QW_ROTARY_SCALE_LINEAR = 1,

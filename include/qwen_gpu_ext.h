@@ -199,7 +199,8 @@ int qw_gpu_attn_block_causal_bounded_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  *   (a, b) <- magnitude * (a cos(pf) - b sin(pf), a sin(pf) + b cos(pf))
  * with p = positions[token] (U32) and f = frequencies[i] (F32 [rotary_dim/2]; see
  * qw_rotary_frequencies_host for the scalings of long contexts); the rest of the head
- * is copied.  p * f is reduced in 64 bits: positions may be anything.  head_dim even, up
+ * is copied.  A token has one position, as text has: tokens of an image in a prompt, which
+ * have a time, a row and a column over sections of the pairs, are not covered.  p * f is reduced in 64 bits: positions may be anything.  head_dim even, up
  * to 512.  Each output may be its own input. */
 enum { QW_ROTARY_NEIGHBOURS = 0, QW_ROTARY_HALVES = 1 };
 int qw_gpu_rotary_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_tensor *key_output,
@@ -243,10 +244,14 @@ int qw_gpu_rotary_append_bf16(h3_gpu *gpu, h3_gpu_tensor *query_output, h3_gpu_t
  * a token sees its sequence's cache rows up to its own.  query, output [tokens, heads, 128];
  * grouped heads as in qw_gpu_flash_sdpa_prefix_bf16; scale positive.  A token that sees
  * nothing, or nothing but scores of minus infinity, stores zeros; NaN in its query or in a
- * key that it sees makes its result NaN.  Cache rows past a sequence's end may hold anything; the values of
- * its new tokens must be finite where an earlier one's result is wanted.  max_new: new
- * tokens of the longest sequence, which only chooses the kernels (a sequence may have
- * more).  The first call makes a workspace of the context: run the op once before
+ * key that it sees makes its result NaN.  Cache rows past a sequence's end may hold
+ * anything; the values of its new tokens must be finite where an earlier one's result is
+ * wanted.  max_new: new tokens of the longest sequence, which only chooses the kernels (a
+ * sequence may have more).  A sequence goes to one of two, whose sums have different
+ * orders: by its own new tokens times heads / kv_heads (up to 16 and more), except that
+ * max_new * heads / kv_heads up to 16, or heads / kv_heads above 128, leaves all to the first,
+ * and a larger max_new a batch of one to the second.  Otherwise results repeat bit for bit.
+ * The first call makes a workspace of the context: run the op once before
  * capturing it. */
 int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu_tensor *query,
                                 const h3_gpu_tensor *key_pages, const h3_gpu_tensor *value_pages,

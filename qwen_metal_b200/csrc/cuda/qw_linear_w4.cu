@@ -10,19 +10,21 @@
 // sums are kept in fp32; scale and zero are applied to them:
 //   s (sum (128 + q) x - (128 + z) sum x), the second sum by an MMA with a matrix of ones.
 // So nothing is rounded before y is, and taking 128 away costs an fp32 sum 2^-24 of 136 |x|, where
-// a rounded weight would cost 2^-9 of its own.
+// a rounded weight would cost up to 2^-8 of its own.
 //
 // The warps of a CTA take the columns in turn, 128 at a time, and add their sums through shared
 // memory in a fixed order.
 //
 // What bounds it: the weights' bytes only in the limit.  One row through 4096 -> 32768 (67 MB, groups of
 // 128) takes 19 us in a chain of layers, 3.6 TB/s; through 4096 -> 6144 (12.6 MB) 5.5 us, 2.4 TB/s: a launch
-// reads its code and first operands (4 us), then a warp has four or eight chunks to go.  13 rows take longer by loads of x from L2
-// and integer work that run beside the MMAs only in part.
+// reads its code and first operands (4 us), then a warp has four or eight chunks to go.  13 rows of
+// 4096 -> 12288, groups of 32, take 17 us (tensor pipe 19 %, issue 28 %): the warps wait for loads, of words two
+// chunks ahead and of x, from L2, where it is used.
 //
 // The shape of a CTA follows the tiles of 16 outputs that an SM gets, so that all are there at once and the
-// few columns a warp has left do not wait for few warps.  Passes of four layers of 4096 columns, groups of
-// 128 / 32, us (warps x tiles of outputs, CTAs that an SM must hold):
+// few columns a warp has left do not wait for few warps.  (It does not look at the columns: the figures are those of
+// 4096 but for one line, and with 1024 half of sixteen warps have no chunk.)  Passes of four layers of 4096 columns,
+// groups of 128 / 32, us (warps x tiles of outputs, CTAs that an SM must hold):
 //   up to 8 rows     2048 outputs   16x1 1  26.0 / 27.9    12x1 2  25.7 / 29.9     8x1 3  26.1 / 33.3
 //                    4096           12x1 2  26.5 / 32.6     8x1 3  27.2 / 38.8    16x1 1  30.5 / 42.0
 //                    6144            8x1 3  30.1 / 39.3     8x2 2  30.9 / 46.5    12x1 2  35.3 / 53.0

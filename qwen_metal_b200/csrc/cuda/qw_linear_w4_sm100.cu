@@ -9,17 +9,18 @@
 // is an A operand of its own, so that no weight is rounded: s (q - 8) has 12 bits and is held whole, as is
 // s (q - z) for whole z; other zero points cost at most 3 * 2^-16 of the weight.  (One bf16 number, 2^-8 of the
 // weight off, is half of the MMAs, but a layer then answers otherwise than with few rows: 412 rows of 4096 x 4096
-// 28 us, begin to submit, as here 36; a sum of random weights' products 0.0022 of its size off and 0.0017, which
+// 28 us between a chain's events, as here 36; a sum of random weights' products 0.0022 of its size off and 0.0017, which
 // is the result's own rounding.)  All of a tile's products are summed in fp32 in TMEM.
 //
 // Warps (384 threads):
 //   0      TMA producer: 128 columns of x and of the weights' words a step
 //   1      MMA issuer, TMEM allocation
 //   4..11  weights: words -> two parts in bf16 -> TMEM; at the end TMEM -> the result
-// What bounds it: the MMAs, 16 to a step of 128 columns.  Each takes some 30 clocks for its A out of TMEM and a
-// half for every row: a step of a 112-row tile 1500 clocks, of a 256-row tile 2800 (4000 rows through
-// 4096 x 12288: 590 us, 0.68 PFLOP/s of the layer, 1.36 of the MMAs).  412 rows of 4096 x 4096: 36 us, begin to
-// submit; 300 rows, a layer of a chain, 29 us.
+// What bounds it: up to 128 rows of a tile a step's chain of waits, words, expansion, TMEM stores and MMAs, which
+// run beside one another only in part: 1400 clocks for 112 rows (412 of 4096 x 4096: tensor pipe 55 % active, issue
+// 38 %, ALU 32 %; 36 us between the events of a chain, 49 from its begin to its submit's end; 300 rows, a layer of
+// a chain, 29).  With 256 rows the MMAs, 16 to a step of 128 columns: 2800 clocks (4000 rows through 4096 x 12288
+// 590 us, 0.68 PFLOP/s of the layer, 1.36 of the MMAs).
 // With whole q - z as A and every group's sums taken out of TMEM and scaled in fp32 four warps do nothing else and
 // every group is a hand-over: 4 layers of those 300 rows took 115 us (groups of 128) and 278 us (of 32), as here
 // 121 and 126; 4000 rows 574 and 1404 us, as here 590 and 610; and a zero point that is not whole is rounded.

@@ -2,8 +2,9 @@
 //
 //   o = softmax(scale * q K^T) V over the cache rows a token sees: those before it and its own.
 //
-// The softmax, the MMAs and the CTA's form are those of qw_attn_sm100.cu (running maximum).  What is
-// different here:
+// The softmax, the MMAs and the CTA's form are those of qw_attn_sm100.cu (running maximum; P rounded to bf16
+// for P V, 2^-8 of a weight at most: what that leaves as a second operand would be half as many MMAs again, and
+// longer in the softmax that bounds the kernel).  What is different here:
 //   rows   The query heads of a kv head, token by token, are the rows of a 128-row sub-tile (as many
 //          whole tokens as fit): K and V are read once for all of them, the causal edge of a chunk cuts
 //          128 / share tokens' tiles and not 128 tokens', and a chunk of 16 tokens fills a sub-tile.
@@ -388,7 +389,9 @@ qw_paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         ctl->wait_cycles = p.wait_cycles > 0 ? p.wait_cycles : kWaitCycles;
     }
     if (warp == kMmaWarp) tmem_alloc<1>(&ctl->tmem_base, kTmemCols);
-    // In this order: the kernel for few rows may run beside this one, on what was there before both.
+    // Always in this order, unlike in other kernels: the kernel for few rows, which the host launches directly behind
+    // this one, reads and writes from its start on and relies on this kernel having waited for all that was before
+    // both.  With the trigger ahead of the wait, or another kernel between the two, it would race with that.
     grid_wait();
     grid_launch_dependents();
     uint32_t index = blockIdx.x;

@@ -13,11 +13,14 @@
 //                  them; S^T becomes P^T by movmatrix.
 // So K and V go from global memory to registers to the tensor cores: no shared memory, no barrier.
 // Cache rows past the sequence's end are not read (what they hold may be anything); masked scores
-// are -inf.  Running maximum and sum are fp32 in the exp2 domain, P is rounded to bf16 for P V.
+// are -inf.  Running maximum and sum are fp32 in the exp2 domain, P is rounded to bf16 for P V: 2^-8 of a
+// weight at most, as in the library's other attention.  (What that leaves as a second operand, which would
+// make it 2^-16, spills registers: 64 sequences of up to 4096 keys, two layers, 240 -> 251 us, 1000 of up to 64,
+// four layers, 208 -> 234.)
 //
-// What bounds it: HBM, once there are some MB to read.  One sequence of 131072 keys (537 MB): 100 us,
-// 5.4 TB/s, 83 % of a plain copy's rate; 64 of up to 4096 keys 120 us (5.6 TB/s).  One of 2000 keys: 21 us
-// of which the chain's ends are 14; 1000 sequences of up to 64 keys 58 us, twice what their bytes take:
+// What bounds it: HBM, once there are some MB to read.  One sequence of 131072 keys (537 MB): 97 us,
+// 5.5 TB/s, 85 % of a plain copy's rate; 64 of up to 4096 keys 120 us (5.6 TB/s).  One of 2000 keys: 20 us
+// between the events of a chain, 28 to 32 from its begin to its submit's end; 1000 sequences of up to 64 keys 58 us, twice what their bytes take:
 // a unit of four tiles is a chain of their loads' latencies.  168 registers a thread keep a tile of K and V
 // of each of 12 warps in flight.
 //

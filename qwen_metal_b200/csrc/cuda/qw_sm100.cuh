@@ -36,7 +36,9 @@ __device__ __forceinline__ bool elect_one() {
 // ---- programmatic dependent launch ------------------------------------------
 // A kernel launched with launch() below may start (barriers, TMEM, descriptors) under the
 // tail of the one before it; it waits for that one's results before it touches global
-// memory.
+// memory.  Two kernels do otherwise, and say why they may: qw_linear_w4.cu asks for its
+// weights in L2 ahead of the wait, and qw_paged_few.cu waits at its end where it runs beside
+// the kernel for chunks.
 __device__ __forceinline__ void grid_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }

@@ -273,7 +273,8 @@ int qw_gpu_paged_attention_bf16(h3_gpu *gpu, h3_gpu_tensor *output, const h3_gpu
     const size_t few_bytes = (qwcu_paged_few_workspace_bytes(sms) + 255) / 256 * 256;
     char *workspace = paged_workspace(gpu, few_bytes, qwcu_paged_chunk_workspace_bytes(sms));
     if (!workspace) return 0;
-    /* Each kernel skips the other's sequences; one sequence alone needs no second kernel. */
+    /* Each kernel skips the other's sequences; one sequence alone needs no second kernel.  Where both run, the one
+     * for few rows follows the one for chunks directly: it relies on that one's wait for what was before. */
     const uint32_t share = heads / kv_heads;
     const int chunks = share <= 128 && (uint64_t)max_new * share > QW_PAGED_FEW_ROWS;
     const uint32_t least_rows = batch == 1 ? 0u : QW_PAGED_FEW_ROWS + 1u;
