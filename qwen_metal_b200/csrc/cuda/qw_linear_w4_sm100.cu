@@ -9,8 +9,8 @@
 // is an A operand of its own, so that no weight is rounded: s (q - 8) has 12 bits and is held whole, as is
 // s (q - z) for whole z; other zero points cost at most 3 * 2^-16 of the weight.  (One bf16 number, 2^-8 of the
 // weight off, is half of the MMAs, but a layer then answers otherwise than with few rows: 412 rows of 4096 x 4096
-// 28 us between a chain's events, as here 36; a sum of random weights' products 0.0022 of its size off and 0.0017, which
-// is the result's own rounding.)  All of a tile's products are summed in fp32 in TMEM.
+// 28 us between a chain's events, as here 36; a sum of random weights' products 0.0022 of its size off and 0.0017,
+// which is the result's own rounding.)  All of a tile's products are summed in fp32 in TMEM.
 //
 // Warps (384 threads):
 //   0      TMA producer: 128 columns of x and of the weights' words a step
@@ -20,10 +20,10 @@
 // run beside one another only in part: 1400 clocks for 112 rows (412 of 4096 x 4096: tensor pipe 55 % active, issue
 // 38 %, ALU 32 %; 36 us between the events of a chain, 49 from its begin to its submit's end; 300 rows, a layer of
 // a chain, 29).  With 256 rows the MMAs, 16 to a step of 128 columns: 2800 clocks (4000 rows through 4096 x 12288
-// 590 us, 0.68 PFLOP/s of the layer, 1.36 of the MMAs).
+// 593 us, 0.68 PFLOP/s of the layer, 1.36 of the MMAs).
 // With whole q - z as A and every group's sums taken out of TMEM and scaled in fp32 four warps do nothing else and
 // every group is a hand-over: 4 layers of those 300 rows took 115 us (groups of 128) and 278 us (of 32), as here
-// 121 and 126; 4000 rows 574 and 1404 us, as here 590 and 610; and a zero point that is not whole is rounded.
+// 121 and 126; 4000 rows 574 and 1404 us, as here 593 and 618; and a zero point that is not whole is rounded.
 // A few tiles would leave SMs idle: up to eight CTAs of a cluster then take a share of the columns each
 // and add their sums through each other's shared memory, in the order of the CTAs (30 rows of 4096 x 4096:
 // 9 us a layer).
@@ -264,8 +264,8 @@ __device__ __forceinline__ T uniform(T v) {
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// The MMAs of half a step's A, 128 columns of one part.  Unrolled, on operands in uniform registers: in a loop over them an MMA took 150 clocks
-// to issue, more than twice its execution.
+// The MMAs of half a step's A, 128 columns of one part.  Unrolled, on operands in uniform registers: in a loop
+// over them an MMA took 150 clocks to issue, more than twice its execution.
 __device__ __forceinline__ void issue_part(uint32_t d, uint32_t a, uint32_t x_lo, uint32_t box, uint32_t idesc,
                                            uint32_t accumulate) {
 #pragma unroll

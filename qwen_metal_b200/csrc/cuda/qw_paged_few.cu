@@ -20,7 +20,8 @@
 //
 // What bounds it: HBM, once there are some MB to read.  One sequence of 131072 keys (537 MB): 97 us,
 // 5.5 TB/s, 85 % of a plain copy's rate; 64 of up to 4096 keys 120 us (5.6 TB/s).  One of 2000 keys: 20 us
-// between the events of a chain, 28 to 32 from its begin to its submit's end; 1000 sequences of up to 64 keys 58 us, twice what their bytes take:
+// between the events of a chain, 28 to 32 from its begin to its submit's end; 1000 sequences of up to 64 keys 58 us,
+// twice what their bytes take:
 // a unit of four tiles is a chain of their loads' latencies.  168 registers a thread keep a tile of K and V
 // of each of 12 warps in flight.
 //
